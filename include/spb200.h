@@ -116,6 +116,36 @@ int  spb_session_decode_greedy(spb_session *s, int32_t token, int n_steps, int32
  * the step on its stream; the sessions must be distinct. */
 int  spb_batch_decode_step(spb_session *const *ss, int B, const int32_t *tokens, float *logits,
                            int32_t *argmax);
+/* What a step hands back; every pointer is a host buffer or NULL. rows: the step's token rows. */
+typedef struct {
+    float   *logits;        /* [rows][n_vocab]: the distribution after each row's token */
+    int32_t *argmax;        /* [rows] its first maximum */
+    float   *logprob;       /* [rows] log probability of each row's own token given what precedes it;
+                             * NaN where the preceding row is not part of the step */
+    float   *entropy;       /* [rows] of the distribution after each row's token, in nats */
+    int32_t  top;           /* alternatives per row, 0..32 */
+    int32_t *top_id;        /* [rows][top] the largest entries, equal ones lowest id first */
+    float   *top_logprob;   /* [rows][top] */
+} spb_step_out;
+/* spb_session_prefill that scores its tokens: the logits stay on the device unless asked for.
+ * logprob[0] is NaN (its predecessor belongs to an earlier call); logprob[i] is log p of tokens[i]
+ * given everything before it (spb_logprobs' rules). */
+int  spb_session_score(spb_session *s, const int32_t *tokens, int n_tok, const spb_step_out *out);
+/* One step over drafted trees of B (1..64) sessions of one model, n_nodes[b] >= 1 tokens each and 64
+ * in all: tokens and parents hold session 0's nodes, then session 1's, and so on; a node's parent is
+ * an earlier node of its session (its index there), or -1 for a token that follows the context
+ * directly. Every node sees its session's context and its own ancestors: its logits are the bytes that
+ * decoding the path to it token by token gives. out (nullable): one row per node. logprob of a node
+ * with parent -1 is NaN. The nodes' K and V rows are cached behind the context (slot position + i),
+ * where they stay until spb_session_tree_commit keeps one path; no position moves, and any other call
+ * that writes the cache, or a rewind, drops the tree. Unpaged and paged sessions, not Spinor ones
+ * (SPB_EUNSUPPORTED). ss[0] runs the step on its stream; the sessions must be distinct. */
+int  spb_batch_tree_step(spb_session *const *ss, int B, const int32_t *n_nodes, const int32_t *tokens,
+                         const int32_t *parents, const spb_step_out *out);
+/* Keep the n nodes of path (path[0] with parent -1, each the child of the one before; n = 0 keeps
+ * none) of the session's last tree step: their K and V rows become the positions that follow the
+ * context, the position advances by n, the rest of the tree is dropped. SPB_EBADSTATE without a tree. */
+int  spb_session_tree_commit(spb_session *s, const int32_t *path, int n);
 int  spb_session_rewind(spb_session *s, int n);          /* O(1): position -= n */
 int  spb_session_position(const spb_session *s);         /* -1 on NULL */
 /* sp_session_clone (sp_session.c:773-816): a session at the same position with the same cache.
@@ -212,6 +242,46 @@ int spb_silu_exact_dev(const float *x, int n, float *out, void *stream);
 /* CORDIC-RoPE of `rows` head vectors of length d at positions pos[r] (device) */
 int spb_rope_cordic_dev(const float *v, int d, int rows, const int32_t *pos, float base,
                         int32_t *out, void *stream);
+/* Caches of several sequences in device memory: pools of n_pages pages [n_layers][n_head_kv][page]
+ * [head_dim] int32 on the 2^16 grid (|k| < 2^24, |v| < 2^30), 16-byte aligned. ptab [n_seq][ptab_ld]
+ * (device): the page of sequence s's positions [j page, (j + 1) page); NULL: sequence s is page s.
+ * Any page >= 1; head_dim 64, 128 or 256. */
+typedef struct {
+    int32_t       *k, *v;
+    const int32_t *ptab;
+    int32_t        n_pages, page, ptab_ld;
+    int32_t        n_layers, n_head_kv, head_dim;
+} spb_kv_view;
+/* Attention of drafted trees over their caches, as in spb_batch_tree_step: the nodes of sequence s are
+ * the rows row0[s] .. row0[s + 1] (64 at most, none is fine), parent[row] a node's parent in its
+ * sequence (an earlier node's index, or -1), ctx[s] the positions its cache holds; node i's K and V
+ * rows are in slot ctx[s] + i already, its position is ctx[s] + its depth. q and out [rows][n_head
+ * head_dim]: rotated queries on the 2^16 grid (|q| < 2^24), f32 outputs. window <= 0: none, else a
+ * node sees the window positions up to its own. max_ctx (host): no ctx[s] is larger. ctx, row0
+ * [n_seq + 1], parent, q, out and the view's pointers are memory of the current device; nothing is
+ * allocated after the first call on a device, calls on different streams are independent. A sequence
+ * whose arrays are out of range raises a bit (spb_take_device_errors) and leaves its rows as they
+ * were, as are rows of no sequence; a page outside the pool raises the bit and reads as page 0. The
+ * bytes are those of decoding each path (sp_session.c:327-347 on the exact islands). */
+int spb_tree_attn(const spb_kv_view *kv, int layer, int n_seq, const int32_t *ctx, const int32_t *row0,
+                  const int32_t *parent, int rows, int max_ctx, const int32_t *q, int n_head, int window,
+                  float *out, void *stream);
+/* In every layer, K and V: slot ctx[s] + path[i] -> slot ctx[s] + i for the accepted nodes path[path0[s]
+ * .. path0[s + 1]] of each sequence (strictly ascending, below 64), in place; device arrays as above,
+ * n_path = path0[n_seq]. The slots' pages must belong to one sequence each. A sequence out of range
+ * (or with a page outside the pool) raises a bit and moves nothing. */
+int spb_kv_compact(const spb_kv_view *kv, int n_seq, const int32_t *ctx, const int32_t *path0,
+                   const int32_t *path, int n_path, void *stream);
+/* Log probabilities over rows of f32 logits [rows][ld], vocab entries each: logprob[t] = x[tok_row[t]]
+ * [tok[t]] - lse (tok_row NULL: row t; tok -1: NaN; any other token or row out of range raises a bit
+ * and gives NaN), lse and entropy [rows] (each NULL: not wanted), and the top (0..32) largest entries'
+ * ids and log probabilities, equal entries lowest id first. -inf entries are masked tokens: logprob
+ * -inf, no alternative (id -1, -inf where a row has fewer than top). A row of -inf alone has lse -inf
+ * and entropy 0; a row with NaN or +inf has no distribution: NaN, ids -1. A row's results do not depend
+ * on the other rows of the call. Device buffers of the current device; no workspace. */
+int spb_logprobs(const float *logits, int rows, int vocab, int64_t ld, const int32_t *tok_row,
+                 const int32_t *tok, int n_tok, float *logprob, float *lse, float *entropy, int top,
+                 int32_t *top_id, float *top_logprob, void *stream);
 /* error bits raised by the last isolated-kernel call on this thread's device */
 int spb_take_device_errors(void);
 

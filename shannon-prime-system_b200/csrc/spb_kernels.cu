@@ -1332,14 +1332,15 @@ __global__ void k_rope_kv(RopeArgs a) {
   const int head = blockIdx.x, t = blockIdx.y;
   const int HD = a.HD, half = HD >> 1, QD = a.NH * HD, KVD = a.NKV * HD;
   const float *row = a.qkv + (size_t)t * (QD + 2 * KVD);
-  int p;
+  int p, ps;   // position (the rotation's) and cache slot
   KvPages kv;
   if (a.rows) {   // row t of a multi-session batch: its own session's position and cache
     const BatchRow br = a.rows[t];
     p = br.pos;
+    ps = br.slot;
     kv = br.kv;
   } else {
-    p = a.pos_dev[0] + t;
+    p = ps = a.pos_dev[0] + t;
     kv = a.kv;
   }
   const int i = threadIdx.x;   // pair index, blockDim.x == half
@@ -1357,14 +1358,14 @@ __global__ void k_rope_kv(RopeArgs a) {
   if (head >= a.NH + a.NKV && spin) {   // V head: Spinor blocks of the float projections
     const int g = head - a.NH - a.NKV;
     spin_encode_row(row + QD + KVD + g * HD, false, HD,
-                    reinterpret_cast<uint8_t *>(kv.v) + kv_spin_off(kv, a.NKV, a.layer, g, p), nullptr, imgs, tab,
+                    reinterpret_cast<uint8_t *>(kv.v) + kv_spin_off(kv, a.NKV, a.layer, g, ps), nullptr, imgs, tab,
                     a.err);
     return;
   }
   if (head >= a.NH + a.NKV) {  // V head: quantize to the 2^16 grid
     const int g = head - a.NH - a.NKV;
     const float *src = row + QD + KVD + g * HD;
-    int32_t *dst = kv.v + kv_elem(kv, a.NL, a.NKV, HD, a.layer, g, p);
+    int32_t *dst = kv.v + kv_elem(kv, a.NL, a.NKV, HD, a.layer, g, ps);
 #pragma unroll
     for (int r = 0; r < 2; r++) {
       const float v = src[i + r * half];
@@ -1394,11 +1395,11 @@ __global__ void k_rope_kv(RopeArgs a) {
     krow[i] = oa;
     krow[i + half] = ob;
     __syncthreads();
-    spin_encode_row(krow, true, HD, reinterpret_cast<uint8_t *>(kv.k) + kv_spin_off(kv, a.NKV, a.layer, hh, p),
+    spin_encode_row(krow, true, HD, reinterpret_cast<uint8_t *>(kv.k) + kv_spin_off(kv, a.NKV, a.layer, hh, ps),
                     nullptr, imgs, tab, a.err);
     return;
   }
-  int32_t *dst = is_q ? a.qi + (size_t)t * QD + hh * HD : kv.k + kv_elem(kv, a.NL, a.NKV, HD, a.layer, hh, p);
+  int32_t *dst = is_q ? a.qi + (size_t)t * QD + hh * HD : kv.k + kv_elem(kv, a.NL, a.NKV, HD, a.layer, hh, ps);
   dst[i] = oa;
   dst[i + half] = ob;
 }

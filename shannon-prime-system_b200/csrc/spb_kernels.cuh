@@ -14,6 +14,7 @@ enum : uint32_t {
   ERR_SCORE_RANGE = 1u << 4,  // |score| >= 2^17
   ERR_TOKEN = 1u << 5,        // token id outside [0, vocab)
   ERR_TIMEOUT = 1u << 6,      // a bounded wait on an asynchronous copy gave up
+  ERR_TREE = 1u << 7,         // a tree's parents, rows, context or path, or a page table entry, out of range
 };
 
 
@@ -136,11 +137,12 @@ __host__ __device__ inline size_t kv_elem(const KvPages &kv, int NL, int NKV, in
   return ((page * NL + L) * NKV + g) * (size_t)kv.pg * HD + (size_t)(p - j * kv.pg) * HD;
 }
 
-// One token row of a multi-session batch: its session's K/V pages, the row's position and the
-// session's capacity P.
+// One token row of a multi-session batch: its session's K/V pages, the row's position, the
+// session's capacity P and the cache slot its K/V rows go to. The slot is the position, except
+// for a drafted tree's nodes, which stand at their depth but are stored in drafting order.
 struct BatchRow {
   KvPages kv;
-  int32_t pos, P;
+  int32_t pos, P, slot;
 };
 
 struct RopeArgs {

@@ -13,6 +13,7 @@
 #include "spb_kernels.cuh"
 #include "spb_spinor.cuh"
 #include "spb_tp.cuh"
+#include "spb_tree.cuh"
 
 #include <cuda_runtime.h>
 
@@ -64,6 +65,7 @@ static const char *err_bits_text(uint32_t b) {
   if (b & ERR_V_RANGE) return "v outside the exact range (|v| < 16384)";
   if (b & ERR_SCORE_RANGE) return "attention score outside the exact range (|z| < 2^17)";
   if (b & ERR_TIMEOUT) return "a bounded wait gave up (timeout)";
+  if (b & ERR_TREE) return "a tree's parents, rows, context or path, or a page table entry, out of range";
   return "unknown";
 }
 
@@ -668,6 +670,13 @@ struct spb_session {
   BatchRow *rows_dev = nullptr;   // [NT_MAX] rows of a multi-session batch led by this session
   BatchRow *h_rows = nullptr;     // pinned staging for rows_dev
   int32_t *h_argmax = nullptr;    // pinned [NT_MAX] batch argmaxes
+  // a step over drafted trees led by this session (behind rows_dev and h_rows): each session's
+  // cache and rows, the nodes' parents, and the row and token of every log probability asked for
+  TreeSeq *trees_dev = nullptr, *h_trees = nullptr;
+  int32_t *nodes_dev = nullptr, *h_nodes = nullptr;   // [3][LG_MAX]: parent (or path), row, token
+  float *lp_dev = nullptr;        // [LG_MAX] logprob, lse, entropy, then [LG_MAX][LOGPROB_TOP] ids and logprobs
+  // the drafted tree cached behind the context, until it is committed or the slots are written again
+  std::vector<int32_t> tree;      // parents
   cudaGraphExec_t step_graph = nullptr;
   size_t buf_bytes = 0;
   // tensor parallel: int64 partial sums of the K-split matrices [NT_MAX][E], this rank's LM-head
@@ -678,6 +687,12 @@ struct spb_session {
   size_t ws_elems = 0;
   unsigned flags = 0;             // SPB_KV_SPINOR: K/V rows kept as Spinor blocks (kv.rb bytes each)
 };
+
+// rows of a batch, then the trees' staging: one region on the device and one pinned on the host
+constexpr size_t ROWS_BYTES = (NT_MAX * sizeof(BatchRow) + 15) / 16 * 16;
+constexpr size_t TREES_BYTES = (LG_MAX * sizeof(TreeSeq) + 15) / 16 * 16;
+constexpr size_t ROWS_STAGE = ROWS_BYTES + TREES_BYTES + 3 * LG_MAX * 4;
+constexpr size_t LP_FLOATS = 3 * LG_MAX + 2 * (size_t)LG_MAX * LOGPROB_TOP;
 
 static size_t kv_layer_elems(const spb_model *m, int pmax) { return (size_t)m->NKV * pmax * m->HD; }
 
@@ -720,7 +735,7 @@ static int session_open(spb_model *m, int pmax, spb_kvpool *pool, spb_session **
   const size_t o_as = take(NT_MAX * 4), o_pos = take(4), o_tok = take(NT_MAX * 4), o_am = take(NT_MAX * 4);
   const size_t o_hist = take((size_t)pmax * 4), o_err = take(4), o_slots = take(2 * NT_MAX * 4);
   const size_t o_keys = take(NT_MAX * 8);
-  const size_t o_rows = take(NT_MAX * sizeof(BatchRow));
+  const size_t o_rows = take(ROWS_STAGE), o_lp = take(LP_FLOATS * 4);
   cudaError_t e = cudaSuccess;
   if (session_reuse_enabled()) {
     // the most recently closed buffer of exactly this size, else the smallest within 25 % above it
@@ -769,6 +784,9 @@ static int session_open(spb_model *m, int pmax, spb_kvpool *pool, spb_session **
   s->ao_max = (uint32_t *)(B + o_slots); s->gg_max = s->ao_max + NT_MAX;
   s->amax_keys = (unsigned long long *)(B + o_keys);
   s->rows_dev = (BatchRow *)(B + o_rows);
+  s->trees_dev = (TreeSeq *)(B + o_rows + ROWS_BYTES);
+  s->nodes_dev = (int32_t *)(B + o_rows + ROWS_BYTES + TREES_BYTES);
+  s->lp_dev = (float *)(B + o_lp);
   s->ws = (int64_t *)(B + o_ws);
   s->ws_elems = (size_t)4 * NT_MAX * E;
   if (m->tp) {
@@ -778,11 +796,13 @@ static int session_open(spb_model *m, int pmax, spb_kvpool *pool, spb_session **
   }
   if (!s->st) e = cudaStreamCreateWithFlags(&s->st, cudaStreamNonBlocking);
   if (e == cudaSuccess && !s->h_pinned) e = cudaMallocHost(&s->h_pinned, (NT_MAX + 4) * 4);
-  if (e == cudaSuccess && !s->h_rows) e = cudaMallocHost(&s->h_rows, NT_MAX * sizeof(BatchRow));
+  if (e == cudaSuccess && !s->h_rows) e = cudaMallocHost(&s->h_rows, ROWS_STAGE);
   if (e == cudaSuccess && !s->h_argmax) e = cudaMallocHost(&s->h_argmax, NT_MAX * 4);
   if (e == cudaSuccess) e = cudaMemsetAsync(s->buf, 0, off, s->st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(s->st);
   if (e != cudaSuccess) { spb_session_close(s); return set_err(SPB_ECUDA, "spb_session_open: %s", cudaGetErrorString(e)); }
+  s->h_trees = (TreeSeq *)((uint8_t *)s->h_rows + ROWS_BYTES);
+  s->h_nodes = (int32_t *)((uint8_t *)s->h_rows + ROWS_BYTES + TREES_BYTES);
   *out = s;
   return SPB_OK;
 }
@@ -813,6 +833,7 @@ static void release_pages(spb_session *s) {
 // follows. A copy is waited for before the other holder may write its page in place again.
 static int prepare_write(spb_session *s, int pos, int n) {
   spb_kvpool *pool = s->pool;
+  s->tree.clear();   // a drafted tree behind the context is written over
   if (!pool || n <= 0) return SPB_OK;
   if (pos < 0 || pos + n > s->pmax) return set_err(SPB_ECONTEXT_FULL, "spb: context full");
   bool changed = false, copied = false;
@@ -930,9 +951,10 @@ static bool rope_fused_enabled() {
 
 // Enqueue the schedule for nt rows (tokens already in tok_dev, positions at pos_dev). With
 // rows (device, [nt]), row t belongs to its own session: RoPE/KV store and attention use that
-// session's cache and position; Pmax is the largest of their capacities.
+// session's cache and position; Pmax is the largest of their capacities. With n_trees, the rows
+// are drafted trees' nodes (trees_dev, their parents in nodes_dev; Pmax: the longest context).
 static cudaError_t enqueue_rows(spb_session *s, int nt, bool want_logits, const BatchRow *rows = nullptr,
-                                int Pmax = 0, bool rows_spin = false) {
+                                int Pmax = 0, bool rows_spin = false, int n_trees = 0) {
   spb_model *m = s->m;
   cudaStream_t st = s->st;
   const int E = m->E, QKV = m->QD + 2 * m->KVD;
@@ -947,7 +969,7 @@ static cudaError_t enqueue_rows(spb_session *s, int nt, bool want_logits, const 
   // rows whose only new position is their own (a decode row, or rows of distinct sessions) get
   // QK-norm, RoPE and the K/V store inside the attention kernel; prefill chunks, whose rows read
   // each other's new K/V, keep the separate k_rope_kv
-  const bool fuse_rope = (nt == 1 || rows != nullptr) && rope_fused_enabled();
+  const bool fuse_rope = (nt == 1 || rows != nullptr) && n_trees == 0 && rope_fused_enabled();
   // a K-split matrix (tensor parallel): exact int64 partial sums, summed over the group, then
   // scaled with the GEMV's own rounding
   auto split_gemv = [&](const DevQ4B &w, float *y) -> cudaError_t {
@@ -989,7 +1011,17 @@ static cudaError_t enqueue_rows(spb_session *s, int nt, bool want_logits, const 
       aa.qkv = s->qkv; aa.q_norm = d.q_norm; aa.k_norm = d.k_norm;
       aa.W = ra.W; aa.T = m->tabs; aa.gain = m->gain;
     }
-    K(launch_attn(aa, st));
+    if (n_trees) {
+      TreeAttnArgs ta{};
+      ta.c.seqs = s->trees_dev; ta.c.n_seq = n_trees; ta.c.rows = nt;
+      ta.c.NL = m->NL; ta.c.NKV = m->NKV; ta.c.HD = m->HD;
+      ta.layer = L; ta.NH = m->NH; ta.win = d.win; ta.max_ctx = Pmax;
+      ta.parent = s->nodes_dev; ta.q = s->qi; ta.out = s->ao;
+      ta.ascale = ascale; ta.err = s->err_dev; ta.ao_max = s->ao_max;
+      K(launch_tree_attn(ta, st));
+    } else {
+      K(launch_attn(aa, st));
+    }
     if (m->tp) K(tp_max_u32(m->tp, s->ao_max, nt, st, s->err_dev));   // the quantizer's max over all heads
     K(launch_quant(s->ao, m->QD, m->QD, nt, s->act, s->ao_max, s->err_dev, st));
     K(split_gemv(d.o, s->ap));
@@ -1141,7 +1173,7 @@ extern "C" int spb_batch_decode_step(spb_session *const *ss, int B, const int32_
   for (int i = 1; i < B; i++) CU(cudaStreamSynchronize(ss[i]->st));   // their caches are settled
   for (int i = 0; i < B; i++) {
     lead->h_pinned[i] = tokens[i];
-    lead->h_rows[i] = BatchRow{ss[i]->kv, ss[i]->pos, ss[i]->pmax};
+    lead->h_rows[i] = BatchRow{ss[i]->kv, ss[i]->pos, ss[i]->pmax, ss[i]->pos};
   }
   CU(cudaMemcpyAsync(lead->tok_dev, lead->h_pinned, (size_t)B * 4, cudaMemcpyHostToDevice, lead->st));
   CU(cudaMemcpyAsync(lead->rows_dev, lead->h_rows, (size_t)B * sizeof(BatchRow), cudaMemcpyHostToDevice, lead->st));
@@ -1159,6 +1191,190 @@ extern "C" int spb_batch_decode_step(spb_session *const *ss, int B, const int32_
   }
   for (int i = 0; i < B; i++) CU(cudaStreamSynchronize(ss[i]->st));
   return SPB_OK;
+}
+
+// ---- log probabilities of a pass's rows (its logits on the device) into the caller's buffers
+static int check_out(const spb_step_out *o, const char *who) {
+  if (!o) return SPB_OK;
+  if (o->top < 0 || o->top > LOGPROB_TOP) return set_err(SPB_EBADARG, "%s: top in [0, %d]", who, LOGPROB_TOP);
+  if (o->top > 0 && (!o->top_id || !o->top_logprob))
+    return set_err(SPB_EBADARG, "%s: top without top_id and top_logprob", who);
+  return SPB_OK;
+}
+
+// rows [0, nt) of s->logits to rows [at, at + nt) of o; n_tok log probabilities of (row, token)
+// pairs staged at nodes_dev + LG_MAX, to o->logprob + lp_at
+static int emit_out(spb_session *s, int nt, int at, int n_tok, int lp_at, const spb_step_out *o) {
+  const size_t V = (size_t)s->m->Vfull;
+  if (o->logits)
+    CU(cudaMemcpyAsync(o->logits + (size_t)at * V, s->logits, (size_t)nt * V * 4, cudaMemcpyDeviceToHost, s->st));
+  if (o->argmax)
+    CU(cudaMemcpyAsync(o->argmax + at, s->argmax_dev, (size_t)nt * 4, cudaMemcpyDeviceToHost, s->st));
+  const bool want_lp = o->logprob && n_tok > 0;
+  if (!want_lp && !o->entropy && o->top == 0) return SPB_OK;
+  LogprobArgs a{};
+  a.x = s->logits; a.rows = nt; a.vocab = s->m->Vfull; a.ld = s->m->Vfull;
+  a.tok_row = s->nodes_dev + LG_MAX; a.tok = s->nodes_dev + 2 * LG_MAX; a.n_tok = want_lp ? n_tok : 0;
+  a.logprob = s->lp_dev; a.lse = nullptr; a.entropy = s->lp_dev + 2 * LG_MAX;
+  a.top = o->top;
+  a.ids = reinterpret_cast<int32_t *>(s->lp_dev + 3 * LG_MAX);
+  a.best = s->lp_dev + 3 * LG_MAX + (size_t)LG_MAX * LOGPROB_TOP;
+  a.err = s->err_dev;
+  CU(launch_logprobs(a, s->st));
+  if (want_lp) CU(cudaMemcpyAsync(o->logprob + lp_at, a.logprob, (size_t)n_tok * 4, cudaMemcpyDeviceToHost, s->st));
+  if (o->entropy) CU(cudaMemcpyAsync(o->entropy + at, a.entropy, (size_t)nt * 4, cudaMemcpyDeviceToHost, s->st));
+  if (o->top) {
+    const size_t n = (size_t)nt * o->top * 4;
+    CU(cudaMemcpyAsync(o->top_id + (size_t)at * o->top, a.ids, n, cudaMemcpyDeviceToHost, s->st));
+    CU(cudaMemcpyAsync(o->top_logprob + (size_t)at * o->top, a.best, n, cudaMemcpyDeviceToHost, s->st));
+  }
+  return SPB_OK;
+}
+
+extern "C" int spb_session_score(spb_session *s, const int32_t *tokens, int n_tok, const spb_step_out *out) {
+  if (!s || !tokens || n_tok <= 0 || !out) return set_err(SPB_EBADARG, "spb_session_score: bad arg");
+  int rc = check_out(out, "spb_session_score");
+  if (rc) return rc;
+  if (n_tok > s->pmax - s->pos) return set_err(SPB_ECONTEXT_FULL, "spb_session_score: context full");
+  CU(cudaSetDevice(s->m->device));
+  const int pos0 = s->pos;
+  rc = prepare_write(s, s->pos, n_tok);
+  if (!rc) rc = sync_pos(s);
+  if (rc) return rc;
+  if (out->logprob) out->logprob[0] = NAN;   // its predecessor's row belongs to an earlier call
+  for (int done = 0; done < n_tok;) {
+    int nt = LG_MAX;
+    while (nt > n_tok - done) nt >>= 1;
+    memcpy(s->h_pinned, tokens + done, (size_t)nt * 4);
+    CU(cudaMemcpyAsync(s->tok_dev, s->h_pinned, (size_t)nt * 4, cudaMemcpyHostToDevice, s->st));
+    const int nlp = std::min(nt, n_tok - done - 1);   // row t against the token that follows it
+    for (int t = 0; t < nlp; t++) {
+      s->h_nodes[LG_MAX + t] = t;
+      s->h_nodes[2 * LG_MAX + t] = tokens[done + t + 1];
+    }
+    CU(cudaMemcpyAsync(s->nodes_dev + LG_MAX, s->h_nodes + LG_MAX, (size_t)2 * LG_MAX * 4, cudaMemcpyHostToDevice,
+                       s->st));
+    CU(enqueue_rows(s, nt, true));
+    CU(launch_advance(s->pos_dev, nt, nullptr, nullptr, s->st));
+    rc = emit_out(s, nt, done, nlp, done + 1, out);
+    if (rc) return rc;
+    CU(cudaStreamSynchronize(s->st));   // the staging is written again by the next chunk
+    done += nt;
+  }
+  rc = collect_errors(s);
+  if (rc) { s->pos = pos0; sync_pos(s); cudaStreamSynchronize(s->st); return rc; }
+  s->pos = pos0 + n_tok;
+  return SPB_OK;
+}
+
+// ---- drafted trees: one pass over every node of every session's tree, the nodes cached behind
+// their contexts; a commit then keeps one path. ss[0] leads, as in spb_batch_decode_step.
+extern "C" int spb_batch_tree_step(spb_session *const *ss, int B, const int32_t *n_nodes, const int32_t *tokens,
+                                   const int32_t *parents, const spb_step_out *out) {
+  if (!ss || !n_nodes || !tokens || !parents || B <= 0 || B > LG_MAX)
+    return set_err(SPB_EBADARG, "spb_batch_tree_step: bad arg (B in [1, %d])", LG_MAX);
+  int rc = check_out(out, "spb_batch_tree_step");
+  if (rc) return rc;
+  spb_session *lead = ss[0];
+  if (!lead) return set_err(SPB_EBADARG, "spb_batch_tree_step: null session");
+  int rows = 0, max_ctx = 0;
+  for (int b = 0; b < B; b++) {
+    spb_session *s = ss[b];
+    if (!s || s->m != lead->m) return set_err(SPB_EBADARG, "spb_batch_tree_step: sessions must share one model");
+    for (int j = 0; j < b; j++)
+      if (ss[j] == s) return set_err(SPB_EBADARG, "spb_batch_tree_step: session %d repeated", b);
+    if (s->kv.rb) return set_err(SPB_EUNSUPPORTED, "spb_batch_tree_step: session %d keeps Spinor K/V", b);
+    if (n_nodes[b] <= 0 || n_nodes[b] > LG_MAX - rows)
+      return set_err(SPB_EBADARG, "spb_batch_tree_step: 1 node at least per session, %d in all at most", LG_MAX);
+    if (n_nodes[b] > s->pmax - s->pos) return set_err(SPB_ECONTEXT_FULL, "spb_batch_tree_step: session %d context full", b);
+    for (int i = 0; i < n_nodes[b]; i++)
+      if (parents[rows + i] < -1 || parents[rows + i] >= i)
+        return set_err(SPB_EBADARG, "spb_batch_tree_step: session %d node %d: its parent must be -1 or an earlier node", b, i);
+    rows += n_nodes[b];
+    max_ctx = std::max(max_ctx, s->pos);
+  }
+  CU(cudaSetDevice(lead->m->device));
+  for (int b = 0; b < B; b++) {
+    rc = prepare_write(ss[b], ss[b]->pos, n_nodes[b]);
+    if (rc) return rc;
+  }
+  for (int b = 1; b < B; b++) CU(cudaStreamSynchronize(ss[b]->st));   // their caches are settled
+  int at = 0, nlp = 0;
+  int lp_of[LG_MAX];   // node of each log probability
+  for (int b = 0; b < B; b++) {
+    spb_session *s = ss[b];
+    int depth[LG_MAX];
+    lead->h_trees[b] = TreeSeq{s->kv, s->pos, at, n_nodes[b], s->pmax};
+    for (int i = 0; i < n_nodes[b]; i++) {
+      const int p = parents[at + i];
+      depth[i] = p < 0 ? 0 : depth[p] + 1;
+      lead->h_pinned[at + i] = tokens[at + i];
+      lead->h_rows[at + i] = BatchRow{s->kv, s->pos + depth[i], s->pmax, s->pos + i};
+      lead->h_nodes[at + i] = p;
+      if (p >= 0) {   // a node's token is scored in its parent's row
+        lead->h_nodes[LG_MAX + nlp] = at + p;
+        lead->h_nodes[2 * LG_MAX + nlp] = tokens[at + i];
+        lp_of[nlp++] = at + i;
+      }
+    }
+    at += n_nodes[b];
+  }
+  CU(cudaMemcpyAsync(lead->tok_dev, lead->h_pinned, (size_t)rows * 4, cudaMemcpyHostToDevice, lead->st));
+  CU(cudaMemcpyAsync(lead->rows_dev, lead->h_rows, ROWS_STAGE, cudaMemcpyHostToDevice, lead->st));
+  CU(enqueue_rows(lead, rows, true, lead->rows_dev, max_ctx, false, B));
+  float lp[LG_MAX];
+  spb_step_out o{};
+  if (out) {
+    o = *out;
+    if (o.logprob) o.logprob = lp;
+    rc = emit_out(lead, rows, 0, nlp, 0, &o);
+    if (rc) return rc;
+  }
+  rc = collect_errors(lead);
+  if (rc) return rc;   // no tree is cached
+  if (out && out->logprob) {
+    for (int i = 0; i < rows; i++) out->logprob[i] = NAN;   // first tokens: their predecessor is no row of this step
+    for (int i = 0; i < nlp; i++) out->logprob[lp_of[i]] = lp[i];
+  }
+  at = 0;
+  for (int b = 0; b < B; b++) {
+    ss[b]->tree.assign(parents + at, parents + at + n_nodes[b]);
+    at += n_nodes[b];
+  }
+  return SPB_OK;
+}
+
+extern "C" int spb_session_tree_commit(spb_session *s, const int32_t *path, int n) {
+  if (!s || n < 0 || (n > 0 && !path)) return set_err(SPB_EBADARG, "spb_session_tree_commit: bad arg");
+  if (s->tree.empty()) return set_err(SPB_EBADSTATE, "spb_session_tree_commit: no tree is cached behind the context");
+  const int nodes = (int)s->tree.size();
+  bool moves = false;
+  for (int i = 0; i < n; i++) {
+    if (path[i] < 0 || path[i] >= nodes || s->tree[path[i]] != (i ? path[i - 1] : -1))
+      return set_err(SPB_EBADARG, "spb_session_tree_commit: path[%d] is no child of the node before it", i);
+    moves |= path[i] != i;
+  }
+  CU(cudaSetDevice(s->m->device));
+  if (moves) {
+    const std::vector<int32_t> tree = s->tree;
+    const int rc = prepare_write(s, s->pos, nodes);   // a clone may share the pages by now
+    s->tree = tree;
+    if (rc) return rc;
+    s->h_trees[0] = TreeSeq{s->kv, s->pos, 0, n, s->pmax};
+    memcpy(s->h_nodes, path, (size_t)n * 4);
+    CU(cudaMemcpyAsync(s->trees_dev, s->h_trees, ROWS_STAGE - ROWS_BYTES, cudaMemcpyHostToDevice, s->st));
+    KvCompactArgs a{};
+    a.c.seqs = s->trees_dev; a.c.n_seq = 1; a.c.rows = n;
+    a.c.NL = s->m->NL; a.c.NKV = s->m->NKV; a.c.HD = s->m->HD;
+    a.path = s->nodes_dev;
+    a.err = s->err_dev;
+    CU(launch_kv_compact(a, s->st));
+  }
+  s->tree.clear();
+  s->pos += n;
+  const int rc = sync_pos(s);
+  if (rc) return rc;
+  return collect_errors(s);
 }
 
 extern "C" int spb_session_decode_greedy(spb_session *s, int32_t token, int n_steps, int32_t *tokens_out) {
@@ -1188,6 +1404,7 @@ extern "C" int spb_session_decode_greedy(spb_session *s, int32_t token, int n_st
 extern "C" int spb_session_rewind(spb_session *s, int n) {
   if (!s) return set_err(SPB_EBADARG, "spb_session_rewind: null session");
   if (n < 0 || n > s->pos) return set_err(SPB_EBADARG, "spb_session_rewind: n > position");
+  s->tree.clear();   // a drafted tree belongs to the position it was drafted at
   s->pos -= n;
   CU(cudaSetDevice(s->m->device));
   int rc = sync_pos(s);
@@ -1552,5 +1769,112 @@ extern "C" int spb_rope_cordic_dev(const float *v, int d, int rows, const int32_
   CU(cudaMemcpyAsync(wb, ht.data(), need, cudaMemcpyHostToDevice, st));
   CU(launch_rope_rows(v, d, rows, pos, (const uint64_t *)wb + 32, (const uint64_t *)wb, gain, out, err, st));
   CU(cudaStreamSynchronize(st));
+  return SPB_OK;
+}
+
+// ---- verifying drafted trees over caches in the caller's memory
+// a device buffer of the current device (a host pointer would fault the GPU)
+static bool on_device(const void *p) {
+  cudaPointerAttributes at{};
+  int dev = 0;
+  if (cudaPointerGetAttributes(&at, p) != cudaSuccess || cudaGetDevice(&dev) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  return at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev);
+}
+
+static int check_view(const spb_kv_view *kv, int n_seq, const char *who) {
+  if (!kv || !kv->k || !kv->v || n_seq < 0 || n_seq > 65535)
+    return set_err(SPB_EBADARG, "%s: bad arg (n_seq in [0, 65535])", who);
+  if (kv->n_pages <= 0 || kv->page <= 0 || kv->n_layers <= 0 || kv->n_head_kv <= 0 || (kv->ptab && kv->ptab_ld <= 0))
+    return set_err(SPB_EBADARG, "%s: non-positive cache dimension", who);
+  if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
+    return set_err(SPB_EUNSUPPORTED, "%s: head_dim %d not in {64,128,256}", who, kv->head_dim);
+  if (!kv->ptab && n_seq > kv->n_pages) return set_err(SPB_EBADARG, "%s: fewer pages than sequences and no page table", who);
+  if (((uintptr_t)kv->k & 15) || ((uintptr_t)kv->v & 15)) return set_err(SPB_EBADARG, "%s: k and v must be 16-byte aligned", who);
+  return SPB_OK;
+}
+
+static bool view_on_device(const spb_kv_view *kv) {
+  return on_device(kv->k) && on_device(kv->v) && (!kv->ptab || on_device(kv->ptab));
+}
+
+static TreeCache view_cache(const spb_kv_view *kv, int n_seq, const int32_t *ctx, const int32_t *row0, int rows) {
+  TreeCache c{};
+  c.k = kv->k; c.v = kv->v; c.ptab = kv->ptab; c.ctx = ctx; c.row0 = row0;
+  c.n_pages = kv->n_pages; c.page = kv->page; c.ptab_ld = kv->ptab_ld;
+  c.n_seq = n_seq; c.rows = rows; c.NL = kv->n_layers; c.NKV = kv->n_head_kv; c.HD = kv->head_dim;
+  return c;
+}
+
+extern "C" int spb_tree_attn(const spb_kv_view *kv, int layer, int n_seq, const int32_t *ctx, const int32_t *row0,
+                             const int32_t *parent, int rows, int max_ctx, const int32_t *q, int n_head, int window,
+                             float *out, void *stream) {
+  int rc = check_view(kv, n_seq, "spb_tree_attn");
+  if (rc) return rc;
+  if (layer < 0 || layer >= kv->n_layers || rows < 0 || rows > (long long)n_seq * TREE_NODES || max_ctx < 0)
+    return set_err(SPB_EBADARG, "spb_tree_attn: bad arg (layer, rows in [0, %d n_seq], max_ctx)", TREE_NODES);
+  if (n_head <= 0 || n_head % kv->n_head_kv || n_head / kv->n_head_kv > 8)
+    return set_err(SPB_EUNSUPPORTED, "spb_tree_attn: n_head/n_head_kv must be an integer <= 8");
+  if (rows == 0) return SPB_OK;
+  if (!ctx || !row0 || !parent || !q || !out) return set_err(SPB_EBADARG, "spb_tree_attn: null arg");
+  if ((uintptr_t)q & 15) return set_err(SPB_EBADARG, "spb_tree_attn: q must be 16-byte aligned");
+  if (!view_on_device(kv) || !on_device(ctx) || !on_device(row0) || !on_device(parent) || !on_device(q) || !on_device(out))
+    return set_err(SPB_EBADARG, "spb_tree_attn: an argument is not memory of the current device");
+  uint8_t *wb;
+  TreeAttnArgs a{};
+  rc = work_get(256, &wb, &a.err);
+  if (rc) return rc;
+  a.c = view_cache(kv, n_seq, ctx, row0, rows);
+  a.layer = layer; a.NH = n_head; a.win = window > 0 ? window : -1; a.max_ctx = max_ctx;
+  a.parent = parent; a.q = q; a.out = out;
+  a.ascale = 1.0f / sqrtf((float)kv->head_dim);
+  CU(launch_tree_attn(a, (cudaStream_t)stream));
+  return SPB_OK;
+}
+
+extern "C" int spb_kv_compact(const spb_kv_view *kv, int n_seq, const int32_t *ctx, const int32_t *path0,
+                              const int32_t *path, int n_path, void *stream) {
+  int rc = check_view(kv, n_seq, "spb_kv_compact");
+  if (rc) return rc;
+  if (n_path < 0 || n_path > (long long)n_seq * TREE_NODES)
+    return set_err(SPB_EBADARG, "spb_kv_compact: n_path in [0, %d n_seq]", TREE_NODES);
+  if (n_path == 0) return SPB_OK;
+  if (!ctx || !path0 || !path) return set_err(SPB_EBADARG, "spb_kv_compact: null arg");
+  if (!view_on_device(kv) || !on_device(ctx) || !on_device(path0) || !on_device(path))
+    return set_err(SPB_EBADARG, "spb_kv_compact: an argument is not memory of the current device");
+  uint8_t *wb;
+  KvCompactArgs a{};
+  rc = work_get(256, &wb, &a.err);
+  if (rc) return rc;
+  a.c = view_cache(kv, n_seq, ctx, path0, n_path);
+  a.path = path;
+  CU(launch_kv_compact(a, (cudaStream_t)stream));
+  return SPB_OK;
+}
+
+extern "C" int spb_logprobs(const float *logits, int rows, int vocab, int64_t ld, const int32_t *tok_row,
+                            const int32_t *tok, int n_tok, float *logprob, float *lse, float *entropy, int top,
+                            int32_t *top_id, float *top_logprob, void *stream) {
+  if (rows < 0 || vocab <= 0 || ld < vocab || n_tok < 0)
+    return set_err(SPB_EBADARG, "spb_logprobs: bad arg (rows, n_tok >= 0, vocab > 0, ld >= vocab)");
+  if (top < 0 || top > LOGPROB_TOP) return set_err(SPB_EBADARG, "spb_logprobs: top in [0, %d]", LOGPROB_TOP);
+  if (rows == 0 && n_tok == 0) return SPB_OK;
+  if (rows == 0 || !logits || (n_tok > 0 && (!tok || !logprob)) || (top > 0 && (!top_id || !top_logprob)))
+    return set_err(SPB_EBADARG, "spb_logprobs: null arg, or tokens without rows");
+  if (!tok_row && n_tok > rows) return set_err(SPB_EBADARG, "spb_logprobs: more tokens than rows and no tok_row");
+  const void *ps[] = {logits, n_tok ? tok_row : nullptr, n_tok ? tok : nullptr, n_tok ? logprob : nullptr,
+                      lse, entropy, top ? top_id : nullptr, top ? top_logprob : nullptr};
+  for (const void *p : ps)
+    if (p && !on_device(p)) return set_err(SPB_EBADARG, "spb_logprobs: an argument is not memory of the current device");
+  uint8_t *wb;
+  LogprobArgs a{};
+  const int rc = work_get(256, &wb, &a.err);
+  if (rc) return rc;
+  a.x = logits; a.rows = rows; a.vocab = vocab; a.ld = ld;
+  a.tok_row = tok_row; a.tok = tok; a.n_tok = n_tok; a.logprob = logprob; a.lse = lse; a.entropy = entropy;
+  a.top = top; a.ids = top_id; a.best = top_logprob;
+  CU(launch_logprobs(a, (cudaStream_t)stream));
   return SPB_OK;
 }

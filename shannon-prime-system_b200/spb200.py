@@ -34,7 +34,8 @@ CORE_SYMBOLS = [
     "spb_tp_shard", "spb_tp_unique_id", "spb_tp_open", "spb_tp_close", "spb_tp_rank", "spb_tp_world",
     "spb_model_synthetic_tp", "spb_model_upload_tp", "spb_tp_p2p_init", "spb_tp_p2p_connect",
     "spb_tp_p2p_loopback", "spb_kvpool_create", "spb_kvpool_free", "spb_kvpool_free_pages",
-    "spb_session_open_paged", "spb_session_open_ex", "spb_session_kv_bytes",
+    "spb_session_open_paged", "spb_session_open_ex", "spb_session_kv_bytes", "spb_session_score",
+    "spb_batch_tree_step", "spb_session_tree_commit", "spb_tree_attn", "spb_kv_compact", "spb_logprobs",
 ]
 L1_SYMBOLS = ["spb_l1_forward", "spb_l1_backend", "spb_l1_kvdecode_table", "spb_l1_kvdecode_clone",
               "spb_l1_set_device", "spb_l1_release_model", "spb_l1_kvdecode_table_ext", "spb_l1_set_kv_pool",
@@ -68,6 +69,17 @@ class Config(C.Structure):
 class ModelDesc(C.Structure):
     _fields_ = [("cfg", Config), ("layers", C.c_void_p), ("token_embd", Q4B),
                 ("output", Q4B), ("output_norm", C.c_void_p)]
+
+
+class KvView(C.Structure):
+    """Caches of several sequences in device memory (spb_kv_view); pointers are addresses, ptab may be None."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("ptab", C.c_void_p), ("n_pages", C.c_int32), ("page", C.c_int32),
+                ("ptab_ld", C.c_int32), ("n_layers", C.c_int32), ("n_head_kv", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class StepOut(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("argmax", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p),
+                ("top", C.c_int32), ("top_id", C.c_void_p), ("top_logprob", C.c_void_p)]
 
 
 _LAYER_MAP = [("attn_norm", "attn_norm"), ("q_norm", "attn_q_norm"), ("k_norm", "attn_k_norm"),
@@ -130,6 +142,12 @@ def load(path: str = CORE_SO):
         "spb_session_decode_step_argmax": ([vp, i32, vp, vp], C.c_int),
         "spb_session_decode_greedy": ([vp, i32, C.c_int, vp], C.c_int),
         "spb_batch_decode_step": ([vp, C.c_int, vp, vp, vp], C.c_int),
+        "spb_session_score": ([vp, vp, C.c_int, vp], C.c_int),
+        "spb_batch_tree_step": ([vp, C.c_int, vp, vp, vp, vp], C.c_int),
+        "spb_session_tree_commit": ([vp, vp, C.c_int], C.c_int),
+        "spb_tree_attn": ([vp, C.c_int, C.c_int, vp, vp, vp, C.c_int, C.c_int, vp, C.c_int, C.c_int, vp, vp], C.c_int),
+        "spb_kv_compact": ([vp, C.c_int, vp, vp, vp, C.c_int, vp], C.c_int),
+        "spb_logprobs": ([vp, C.c_int, C.c_int, i64, vp, vp, C.c_int, vp, vp, vp, C.c_int, vp, vp, vp], C.c_int),
         "spb_session_rewind": ([vp, C.c_int], C.c_int), "spb_session_position": ([vp], C.c_int),
         "spb_session_clone": ([vp, C.POINTER(vp)], C.c_int), "spb_session_close": ([vp], None),
         "spb_session_kv_read": ([vp, C.c_int, C.c_int, C.c_int, vp], C.c_int),
@@ -358,6 +376,22 @@ class Session:
         check(load().spb_session_decode_greedy(self.h, int(token), n, out.ctypes.data))
         return out
 
+    def score(self, tokens, top=0, logits=False):
+        """Prefill that scores its tokens: a StepResult, logprob[i] = log p(tokens[i] | all before), NaN for i = 0."""
+        tokens = np.ascontiguousarray(tokens, np.int32)
+        r = StepResult(tokens.size, self.V, top, logits)
+        check(load().spb_session_score(self.h, tokens.ctypes.data, tokens.size, C.byref(r.out)))
+        return r
+
+    def tree_step(self, tokens, parents, top=0, logits=True):
+        """batch_tree_step for this session's tree alone."""
+        return batch_tree_step([self], [tokens], [parents], top, logits)[0]
+
+    def tree_commit(self, path):
+        """Keep the path's nodes of the last tree step; the position advances by their number."""
+        path = np.ascontiguousarray(path, np.int32)
+        check(load().spb_session_tree_commit(self.h, path.ctypes.data, path.size))
+
     def rewind(self, n):
         check(load().spb_session_rewind(self.h, n))
 
@@ -404,6 +438,58 @@ def batch_decode(sessions, tokens, logits=True):
     check(load().spb_batch_decode_step(hs, B, tok.ctypes.data, lg.ctypes.data if logits else None,
                                        am.ctypes.data))
     return lg, am
+
+
+class StepResult:
+    """A step's rows on the host: logits (or None), argmax, logprob, entropy, top_id, top_logprob."""
+
+    def __init__(self, rows, V, top=0, logits=False):
+        self.logits = np.empty((rows, V), np.float32) if logits else None
+        self.argmax = np.empty(rows, np.int32)
+        self.logprob, self.entropy = np.empty(rows, np.float32), np.empty(rows, np.float32)
+        self.top_id, self.top_logprob = np.empty((rows, top), np.int32), np.empty((rows, top), np.float32)
+        self.out = StepOut(_ptr(self.logits), _ptr(self.argmax), _ptr(self.logprob), _ptr(self.entropy), top,
+                           _ptr(self.top_id) if top else None, _ptr(self.top_logprob) if top else None)
+
+    def rows(self, a, b):
+        """The rows [a, b) as a result of their own (views)."""
+        r = object.__new__(StepResult)
+        for f in ("logits", "argmax", "logprob", "entropy", "top_id", "top_logprob"):
+            v = getattr(self, f)
+            setattr(r, f, None if v is None else v[a:b])
+        return r
+
+
+def batch_tree_step(sessions, tokens, parents, top=0, logits=True):
+    """One step over drafted trees of several sessions (spb_batch_tree_step): tokens and parents are one
+    sequence per session; returns one StepResult per session, a row per node."""
+    B = len(sessions)
+    hs = (C.c_void_p * B)(*[s.h for s in sessions])
+    n = np.array([len(t) for t in tokens], np.int32)
+    if [len(p) for p in parents] != n.tolist() or len(tokens) != B:
+        raise ValueError("one parent per token and one tree per session")
+    tok = np.ascontiguousarray(np.concatenate([np.asarray(t, np.int32) for t in tokens]))
+    par = np.ascontiguousarray(np.concatenate([np.asarray(p, np.int32) for p in parents]))
+    r = StepResult(tok.size, sessions[0].V, top, logits)
+    check(load().spb_batch_tree_step(hs, B, n.ctypes.data, tok.ctypes.data, par.ctypes.data, C.byref(r.out)))
+    ends = np.cumsum(n)
+    return [r.rows(e - k, e) for e, k in zip(ends, n)]
+
+
+def tree_attn(kv, layer, n_seq, ctx, row0, parent, rows, max_ctx, q, n_head, window, out, stream=None):
+    """Attention of drafted trees over the caches of a KvView (spb_tree_attn); device addresses."""
+    check(load().spb_tree_attn(C.byref(kv), layer, n_seq, ctx, row0, parent, rows, max_ctx, q, n_head, window, out, stream))
+
+
+def kv_compact(kv, n_seq, ctx, path0, path, n_path, stream=None):
+    """Accepted nodes' K/V rows to the slots behind their contexts, in place (spb_kv_compact)."""
+    check(load().spb_kv_compact(C.byref(kv), n_seq, ctx, path0, path, n_path, stream))
+
+
+def logprobs(logits, rows, vocab, ld, tok_row, tok, n_tok, logprob, lse, entropy, top, top_id, top_logprob, stream=None):
+    """Log probabilities, entropies and alternatives of rows of logits (spb_logprobs); device addresses."""
+    check(load().spb_logprobs(logits, rows, vocab, ld, tok_row, tok, n_tok, logprob, lse, entropy, top, top_id,
+                              top_logprob, stream))
 
 
 class PreparedQ4B:
