@@ -243,7 +243,7 @@ int spb_silu_exact_dev(const float *x, int n, float *out, void *stream);
 int spb_rope_cordic_dev(const float *v, int d, int rows, const int32_t *pos, float base,
                         int32_t *out, void *stream);
 /* Caches of several sequences in device memory: pools of n_pages pages [n_layers][n_head_kv][page]
- * [head_dim] int32 on the 2^16 grid (|k| < 2^24, |v| < 2^30), 16-byte aligned. ptab [n_seq][ptab_ld]
+ * [head_dim] int32 on the 2^16 grid (|k| < 2^24, |v| < 2^30), 32-byte aligned. ptab [n_seq][ptab_ld]
  * (device): the page of sequence s's positions [j page, (j + 1) page); NULL: sequence s is page s.
  * Any page >= 1; head_dim 64, 128 or 256. */
 typedef struct {
@@ -257,7 +257,8 @@ typedef struct {
  * sequence (an earlier node's index, or -1), ctx[s] the positions its cache holds; node i's K and V
  * rows are in slot ctx[s] + i already, its position is ctx[s] + its depth. q and out [rows][n_head
  * head_dim]: rotated queries on the 2^16 grid (|q| < 2^24), f32 outputs. window <= 0: none, else a
- * node sees the window positions up to its own. max_ctx (host): no ctx[s] is larger. ctx, row0
+ * node sees the window positions up to its own. max_ctx (host): no ctx[s] is larger; it, or the window
+ * where that is shorter, is at most 1048512 (SPB_EUNSUPPORTED). ctx, row0
  * [n_seq + 1], parent, q, out and the view's pointers are memory of the current device; nothing is
  * allocated after the first call on a device, calls on different streams are independent. A sequence
  * whose arrays are out of range raises a bit (spb_take_device_errors) and leaves its rows as they

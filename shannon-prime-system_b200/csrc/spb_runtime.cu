@@ -1792,7 +1792,7 @@ static int check_view(const spb_kv_view *kv, int n_seq, const char *who) {
   if (kv->head_dim != 64 && kv->head_dim != 128 && kv->head_dim != 256)
     return set_err(SPB_EUNSUPPORTED, "%s: head_dim %d not in {64,128,256}", who, kv->head_dim);
   if (!kv->ptab && n_seq > kv->n_pages) return set_err(SPB_EBADARG, "%s: fewer pages than sequences and no page table", who);
-  if (((uintptr_t)kv->k & 15) || ((uintptr_t)kv->v & 15)) return set_err(SPB_EBADARG, "%s: k and v must be 16-byte aligned", who);
+  if (((uintptr_t)kv->k & 31) || ((uintptr_t)kv->v & 31)) return set_err(SPB_EBADARG, "%s: k and v must be 32-byte aligned", who);
   return SPB_OK;
 }
 
@@ -1817,6 +1817,8 @@ extern "C" int spb_tree_attn(const spb_kv_view *kv, int layer, int n_seq, const 
     return set_err(SPB_EBADARG, "spb_tree_attn: bad arg (layer, rows in [0, %d n_seq], max_ctx)", TREE_NODES);
   if (n_head <= 0 || n_head % kv->n_head_kv || n_head / kv->n_head_kv > 8)
     return set_err(SPB_EUNSUPPORTED, "spb_tree_attn: n_head/n_head_kv must be an integer <= 8");
+  if ((window > 0 ? std::min(window, max_ctx) : max_ctx) > TREE_SPAN - TREE_NODES)
+    return set_err(SPB_EUNSUPPORTED, "spb_tree_attn: %d visible positions at most", TREE_SPAN - TREE_NODES);
   if (rows == 0) return SPB_OK;
   if (!ctx || !row0 || !parent || !q || !out) return set_err(SPB_EBADARG, "spb_tree_attn: null arg");
   if ((uintptr_t)q & 15) return set_err(SPB_EBADARG, "spb_tree_attn: q must be 16-byte aligned");

@@ -9,7 +9,10 @@
 #include "spb_exact.cuh"
 #include "spb_tree.cuh"
 
+#include <cooperative_groups.h>
 #include <cstdlib>
+
+namespace cg = cooperative_groups;
 
 namespace spb {
 
@@ -48,95 +51,621 @@ __device__ __forceinline__ size_t tree_row(const TreeCache &c, const KvPages &kv
   return ((((size_t)page * c.NL + layer) * c.NKV + g) * kv.pg + (size_t)(slot - j * kv.pg)) * c.HD;
 }
 
-constexpr int TT = 256;
+// ---- exact products on the matrix units
+//
+// An int32 x is four balanced base-256 digits, x = sum_i d_i 256^i with d_i in [-128, 127]: adding
+// 0x80808080 makes every digit u_i = d_i + 128 an unsigned byte (the carries are the balancing).
+// <q, k> = sum_ij 256^(i+j) <digit i of q, digit j of k>, each an int8 matrix product into int32;
+// products of the same i + j share one accumulator (a class). The queries' digits are signed, the
+// cache's lower three stay biased, and the bias comes off once per sum:
+//   <q, k> = sum_i sum_{j<3} 256^(i+j) <d_i(q), u_j(k)> + (fourth digits of k) - BIAS sum q.
+// The exponentials e in [0, 2^30] are four unsigned bytes, so the V-sums' bias is BIAS sum e. A fourth
+// digit that is zero throughout an operand (|x| < 127.5 2^16 on the grid) adds nothing and is skipped.
+// Classes: 3 * 128 * 255 * 256 < 2^25 for a score, (3 * 255 + 128) * 255 per slot of a V-sum.
+constexpr int64_t BIAS = 128 * (1 + 256 + 65536);
 
-// One CTA per (row, head): the window's scores for their maximum, then again in runs of 256 slots
-// for the exponentials and the V-sums.
-__global__ void __launch_bounds__(TT) k_tree_attn(TreeAttnArgs a) {
-  __shared__ int seq_sh;
+// byte planes of four int32 values x + 0x80808080: byte i of out[p] is biased digit p of the i-th value
+__device__ __forceinline__ void digits(int x0, int x1, int x2, int x3, uint32_t (&out)[4]) {
+  const uint32_t w0 = (uint32_t)x0 + 0x80808080u, w1 = (uint32_t)x1 + 0x80808080u;
+  const uint32_t w2 = (uint32_t)x2 + 0x80808080u, w3 = (uint32_t)x3 + 0x80808080u;
+  const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140);
+  const uint32_t c = __byte_perm(w0, w1, 0x7362), d = __byte_perm(w2, w3, 0x7362);
+  out[0] = __byte_perm(a, b, 0x5410);
+  out[1] = __byte_perm(a, b, 0x7632);
+  out[2] = __byte_perm(c, d, 0x5410);
+  out[3] = __byte_perm(c, d, 0x7632) ^ 0x80808080u;   // signed
+}
+__device__ __forceinline__ uint4 bytes4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
+  const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140);
+  const uint32_t c = __byte_perm(w0, w1, 0x7362), d = __byte_perm(w2, w3, 0x7362);
+  return make_uint4(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632), __byte_perm(c, d, 0x5410),
+                    __byte_perm(c, d, 0x7632));
+}
+
+__device__ __forceinline__ void mma_ss(int32_t (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_su(int32_t (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_us(int32_t (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_uu(int32_t (&c)[4], const uint4 &a, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+// 32 bytes of a row in one load: a quad of lanes takes a whole 128-byte line
+__device__ __forceinline__ void ld_kv8(int4 &a, int4 &b, const int32_t *p) {
+  asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+               : "l"(p));
+}
+template <int N>
+__device__ __forceinline__ void ld_kv(int32_t (&v)[N], const int32_t *p) {
+  static_assert(N == 1 || N == 2, "one or two columns");
+  if (N == 2) asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[N - 1]) : "l"(p));
+  else asm volatile("ld.global.b32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+}
+
+constexpr int32_t UNSEEN = INT32_MIN;   // the score of a position that a node does not see
+
+// exp_fixed of a score's distance below its maximum in 32-bit steps: far = max - z in units of 2^-14,
+// g = ceil(far log2(e)) in 2^30, n = g >> 30 octaves and the rest; the island's polynomial in x = 2^30 -
+// rest, each (acc x) >> 30 as the high word of acc * 4x (x < 2^30 here). 363410 steps are 32 octaves, the
+// island's zero.
+__device__ __forceinline__ uint32_t mad_hi(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t d;
+  asm("mad.hi.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t exp_grid(int32_t z, int32_t mx) {
+  const uint32_t far = (uint32_t)mx - (uint32_t)z;
+  const uint64_t g = (uint64_t)far * (uint32_t)K_LOG2E + 16383u;   // 2^44 per octave
+  const uint32_t n = (uint32_t)(g >> 44), r4 = (uint32_t)(g >> 12) & ~3u, x4 = 0u - r4;
+  uint32_t acc = mad_hi(165394u, x4, 1431680u);
+  acc = mad_hi(acc, x4, 10327387u);
+  acc = mad_hi(acc, x4, 59597083u);
+  acc = mad_hi(acc, x4, 257941248u);
+  acc = mad_hi(acc, x4, 744261118u);
+  acc = mad_hi(acc, x4, 1073741824u) >> 1;
+  acc = (r4 == 0u ? 1u << 30 : acc) >> (n & 31u);
+  return z == UNSEEN || far >= 363410u ? 0u : acc;
+}
+
+// f32 of floor(N 2^16 / S) 2^-32 (the decode attention's rounding), r = 2^16 / S in double: N r is off by
+// at most 2^-50 of itself, so its floor is the quotient's unless a whole number lies that near; those, and
+// quotients beyond 2^50, take the exact division.
+__device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
+  const double nd = (int64_t)N.lo >> 63 == N.hi ? __ll2double_rn((int64_t)N.lo)
+                                                : __dadd_rn(__dmul_rn(__ll2double_rn(N.hi), 0x1p64), __ull2double_rn(N.lo));
+  const double x = __dmul_rn(nd, r), w = floor(x), f = __dsub_rn(x, w), eps = __dmul_rn(fabs(x), 0x1p-50);
+  if (f > eps && f < __dsub_rn(1.0, eps) && fabs(x) < 0x1p50) return __double2float_rn(__dmul_rn(w, 0x1p-32));
+  const int64_t hi = (int64_t)(((uint64_t)N.hi << 16) | (N.lo >> 48));   // |N| < 2^80
+  return __double2float_rn(__dmul_rn(__ll2double_rn(floordiv_s128(hi, N.lo << 16, S)), 0x1p-32));
+}
+
+// One CTA: MT * 16 query vectors (a sequence's nodes x the G query heads of one KV head) over a run
+// of slots; a cluster of CL CTAs covers the sequence's slots and joins maxima, sums and V-sums,
+// which are whole numbers, so no split changes a byte.
+//   scores    a warp takes 8 slots at a time: their K rows go from global memory straight into the
+//             column operand (a lane's 32 bytes are eight columns of one slot, so the digit planes
+//             are a byte transpose in registers), the queries' planes wait in shared memory
+//   exps      in place over the scores, each four neighbours' bytes transposed into the planes of
+//             the row operand
+//   V-sums    a warp takes 8 or 16 head dims over all slots of the run, V rows again straight from
+//             global memory (eight slots x one or two dims per lane and step)
+// MULTI (more slots per rank than scores are kept for): the maxima first, then scores again in runs of
+// CS slots, each run's V-sums added up in shared memory.
+template <int HD, int MT, bool MULTI>
+struct TreeTile {
+  static constexpr int QV = 16 * MT, KS = HD / 32;
+  static constexpr int NW = 16, TT = 32 * NW;
+  static constexpr int ND = 2 / MT;                             // head dims of a lane's V rows: its 56 sums
+  static constexpr int DP = HD < 8 * ND * NW ? HD : 8 * ND * NW;   // head dims of one V pass
+  static constexpr int DG = DP / (8 * ND), PG = NW / DG;        // warps along them, groups along the slots
+  static constexpr int PASSES = HD / DP;
+  // slots whose scores are kept (their rows' stride is 16 words off a multiple of 32: no bank conflicts)
+  static constexpr int CS = MULTI ? 1056 : MT == 1 ? 2112 : 1088, SCS = CS + 16;
+  static constexpr size_t QF = (size_t)MT * KS * 4 * 512;       // the queries' planes
+  static constexpr size_t SUMS = (size_t)QV * HD * 16;          // V-sums of a tile
+  // V-sums of the passes before the last (over the planes, not needed by then), or MULTI's running ones
+  static constexpr size_t KEEP = MULTI ? SUMS : (size_t)(PASSES - 1) * QV * DP * 16;
+  static constexpr size_t HEAD = MULTI ? KEEP + QF : (KEEP > QF ? KEEP : QF);
+  static constexpr size_t SC = (size_t)QV * SCS * 4;
+  static constexpr size_t WORK = SC + CS * 4;
+  static constexpr size_t POST = SUMS * (MULTI ? 1 : PG);       // over the scores: every source's sums of this rank's dims
+  static constexpr size_t SMEM = HEAD + (WORK > POST ? WORK : POST);
+};
+
+template <int HD, int MT, bool MULTI>
+__global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
+  using T = TreeTile<HD, MT, MULTI>;
+  constexpr int QV = T::QV, KS = T::KS, SCS = T::SCS, CS = T::CS, TT = T::TT, NW = T::NW, ND = T::ND;
+  constexpr int KG = KS < 4 ? KS : 4;                           // 32-column steps of K loaded at a time
+  extern __shared__ __align__(128) uint8_t raw[];
+  longlong2 *keep = reinterpret_cast<longlong2 *>(raw);         // [QV][DP] per pass, MULTI: [QV][HD]
+  uint4 *qf = reinterpret_cast<uint4 *>(raw + (MULTI ? T::KEEP : 0));   // [MT][KS][4][32]
+  int32_t *sc = reinterpret_cast<int32_t *>(raw + T::HEAD);     // [QV][SCS]
+  uint32_t *rows = reinterpret_cast<uint32_t *>(raw + T::HEAD + T::SC);  // [CS] the slots' rows in K and V
+  longlong2 *sums = reinterpret_cast<longlong2 *>(raw + T::HEAD);        // [CL][PG][QV][HD / CL]
   __shared__ int32_t par[TREE_NODES];
   __shared__ unsigned long long anc[TREE_NODES];
-  __shared__ int32_t qs[256];
-  __shared__ int32_t es[TT];
-  __shared__ int32_t mx;
-  __shared__ unsigned long long ssum;
-  const int row = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int HD = a.c.HD, g = h / (a.NH / a.c.NKV);
+  __shared__ int32_t first[QV];
+  __shared__ unsigned long long seen[QV];
+  __shared__ int32_t bounds[2];                                 // the tile's first slot, its latest window start
+  __shared__ int32_t mx[QV], mx_in[16][QV];
+  __shared__ long long ssum[QV], s_in[16][QV];
+  __shared__ unsigned long long qsum[QV];
+  __shared__ uint32_t omx[QV];
+  __shared__ double rinv[QV];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n8 = lane >> 2, c4 = lane & 3;
+  const int rank = CL > 1 ? (int)cluster.block_rank() : 0, g = blockIdx.y;
+  const int G = a.NH / a.c.NKV;
   pdl_trigger();
+  if (tid < QV) { mx[tid] = UNSEEN; ssum[tid] = 0; qsum[tid] = 0; omx[tid] = 0u; }
   pdl_wait();
-  if (tid == 0) { seq_sh = -1; mx = INT32_MIN; ssum = 0ull; }
-  __syncthreads();
+
+  // ---- which sequence: tiles are counted over the sequences in order (every warp for itself)
   TreeSeq q;
-  for (int s = tid; s < a.c.n_seq; s += TT)
-    if (tree_seq(a.c, s, a.max_ctx, q)) { if (row >= q.row0 && row < q.row0 + q.n) seq_sh = s; }
-    else raise_err(a.err, ERR_TREE);
-  __syncthreads();
-  if (seq_sh < 0) return;
-  tree_seq(a.c, seq_sh, a.max_ctx, q);
-  const int node = row - q.row0;
-  bool bad = false;
-  if (tid < q.n) {
-    const int p = a.parent[q.row0 + tid];
-    bad = p < -1 || p >= tid;
-    par[tid] = p;
+  int tile = -1;
+  for (int s0 = 0, before = 0; s0 < a.c.n_seq; s0 += 32) {
+    int n = 0;
+    if (s0 + lane < a.c.n_seq) {
+      if (tree_seq(a.c, s0 + lane, a.max_ctx, q)) n = (q.n * G + QV - 1) / QV;
+      else if (warp == 0) raise_err(a.err, ERR_TREE);
+    }
+    int incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    const int z = (int)blockIdx.z - before - (incl - n);
+    const uint32_t hit = __ballot_sync(0xffffffffu, z >= 0 && z < n);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      tile = __shfl_sync(0xffffffffu, z, l);
+      tree_seq(a.c, s0 + l, a.max_ctx, q);
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
   }
-  for (int i = tid; i < HD; i += TT) qs[i] = a.q[((size_t)row * a.NH + h) * HD + i];
-  if (__syncthreads_or(bad)) {
+  if (tile < 0) return;   // (the whole cluster)
+  const int x0 = tile * QV, nq = min(QV, q.n * G - x0);   // this tile's query vectors: x -> node x / G, head x % G
+
+  // ---- warp 0: ancestors by doubling, then every query vector's window and tree slots
+  bool bad = false;
+  if (warp == 0) {
+    int up[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int node = lane + 32 * i;
+      up[i] = node < q.n ? a.parent[q.row0 + node] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const int node = lane + 32 * i;
+      if (up[i] < -1 || up[i] >= node) { bad = node < q.n; up[i] = -1; }
+      par[node] = up[i];
+      anc[node] = (1ull << node) | (up[i] >= 0 ? 1ull << up[i] : 0ull);
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    __syncwarp();
+    for (int r = 1; r < q.n; r <<= 1) {
+      unsigned long long m[2];
+      int p[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        m[i] = up[i] >= 0 ? anc[up[i]] : 0ull;
+        p[i] = up[i] >= 0 ? par[up[i]] : -1;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        anc[lane + 32 * i] |= m[i];
+        par[lane + 32 * i] = up[i] = p[i];
+      }
+      __syncwarp();
+    }
+    int f = q.ctx, lo = q.ctx, hi = 0;
+    unsigned long long m = 0;
+    if (lane < nq) {
+      m = anc[(x0 + lane) / G];
+      const int depth = __popcll(m) - 1;
+      f = a.win < 0 ? 0 : max(0, q.ctx + depth - a.win + 1);
+      if (f > q.ctx)   // the window leaves ancestors out
+        for (unsigned long long b = m; b; b &= b - 1) {
+          const int j = __ffsll((long long)b) - 1;
+          if (q.ctx + __popcll(anc[j]) - 1 < f) m &= ~(1ull << j);
+        }
+      lo = min(f, q.ctx);
+      hi = f;
+    }
+    if (lane < QV) {
+      first[lane] = f;
+      seen[lane] = m;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (lane == 0) { bounds[0] = bad ? -1 : lo; bounds[1] = hi; }
+  }
+  // ---- the other warps: the queries' digit planes in the row operand's order, and their sums
+  bool top = false;
+  if (warp > 0)
+    for (int i = tid - 32; i < MT * KS * 32; i += TT - 32) {
+      const int l = i & 31, ks = (i >> 5) % KS, mt = (i >> 5) / KS;
+      uint32_t pl[4][4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {   // (row, columns): the operand's four registers
+        const int x = mt * 16 + (l >> 2) + (u & 1) * 8, d = ks * 32 + (l & 3) * 8 + (u >> 1) * 4;
+        int4 v = make_int4(0, 0, 0, 0);
+        if (x < nq) {
+          const int node = (x0 + x) / G, h = (x0 + x) % G;
+          v = *reinterpret_cast<const int4 *>(a.q + ((size_t)(q.row0 + node) * a.NH + (size_t)g * G + h) * HD + d);
+        }
+        digits(v.x, v.y, v.z, v.w, pl[u]);
+#pragma unroll
+        for (int p = 0; p < 3; p++) pl[u][p] ^= 0x80808080u;
+        top |= pl[u][3] != 0u;
+        int64_t s = (int64_t)v.x + v.y + (int64_t)v.z + v.w;   // of the row's four lanes
+        s += __shfl_xor_sync(0xffffffffu, s, 1);
+        s += __shfl_xor_sync(0xffffffffu, s, 2);
+        if ((l & 3) == 0 && s != 0) atomicAdd(&qsum[x], (unsigned long long)s);
+      }
+#pragma unroll
+      for (int p = 0; p < 4; p++) qf[((mt * KS + ks) * 4 + p) * 32 + l] = make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
+    }
+  const bool q3 = __syncthreads_or(top);   // some query has a fourth digit
+  if (bounds[0] < 0) {   // the parents are out of range (for the whole cluster)
     if (tid == 0) raise_err(a.err, ERR_TREE);
     return;
   }
-  if (tid < q.n) {
-    unsigned long long m = 0;
-    for (int p = tid; p >= 0; p = par[p]) m |= 1ull << p;
-    anc[tid] = m;
-  }
-  __syncthreads();
-  const int depth = __popcll(anc[node]) - 1;
-  const int first = a.win < 0 ? 0 : max(0, q.ctx + depth - a.win + 1);
-  const int end = q.ctx + q.n;
-  auto sees = [&](int slot) {
-    if (slot < q.ctx) return slot >= first;
-    const int i = slot - q.ctx;
-    return ((anc[node] >> i) & 1ull) != 0 && q.ctx + __popcll(anc[i]) - 1 >= first;
+  if (CL > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int u0 = bounds[0], u1 = q.ctx + q.n, clear = bounds[1];
+  const int span = ((u1 - u0 + CL - 1) / CL + 31) & ~31;        // this rank's slots [c0, c1)
+  const int c0 = min(u0 + rank * span, u1), c1 = min(c0 + span, u1);
+
+  auto locate = [&](int cb, int len) {   // the rows of slots [cb, cb + len), the last one again up to a multiple of 32
+    for (int i = tid; i < ((len + 31) & ~31); i += TT)
+      rows[i] = (uint32_t)(tree_row(a.c, q.kv, a.layer, g, cb + min(i, len - 1), a.err) / HD);
+    __syncthreads();
   };
-  auto score = [&](int slot) -> int32_t {   // by one warp
-    const int32_t *kr = q.kv.k + tree_row(a.c, q.kv, a.layer, g, slot, a.err);
-    int64_t s = 0;
-    for (int i = lane; i < HD; i += 32) s += (int64_t)qs[i] * kr[i];
-    s = warp_sum_i64(s);
-    float z = __fmul_rn(__double2float_rn(__dmul_rn(__ll2double_rn(s), 0x1p-32)), a.ascale);
-    if (!(fabsf(z) < 131072.0f)) { raise_err(a.err, ERR_SCORE_RANGE); z = 0.0f; }
-    return (int32_t)llround_d((double)z * 16384.0);
-  };
-  const int u0 = min(first, q.ctx);
-  for (int j = u0 + warp; j < end; j += TT / 32)
-    if (sees(j)) {
-      const int32_t zi = score(j);
-      if (lane == 0) atomicMax(&mx, zi);
+
+  // ---- scores of slots [cb, cb + len) into sc, the rows' maxima into mx
+  auto scores = [&](int cb, int len, bool want_max) {
+    const int nt = ((len + 31) & ~31) / 8;
+    int32_t lmax[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; m++) lmax[m][0] = lmax[m][1] = UNSEEN;
+    // a warp's K rows come in runs of up to four steps (4 KB), which wait as one: the next run leaves once
+    // this one is multiplied, and the SM's other fifteen warps' runs fill the time
+    int4 kb[KG][2];
+    auto load = [&](const int32_t *p) {
+#pragma unroll
+      for (int i = 0; i < KG; i++) ld_kv8(kb[i][0], kb[i][1], p + i * 32);
+    };
+    auto row_of = [&](int t) { return q.kv.k + (size_t)rows[t * 8 + n8] * HD + 8 * c4; };
+    const float scale = __fmul_rn(a.ascale, 0x1p-18f);   // score on the 2^32 grid -> units of 2^-14
+    const int32_t *kr = q.kv.k;
+    if (warp < nt) {
+      kr = row_of(warp);
+      load(kr);
     }
-  __syncthreads();
-  acc128 acc{0ull, 0ll};
-  for (int j0 = u0; j0 < end; j0 += TT) {
-    for (int j = warp; j < TT; j += TT / 32) {
-      int64_t e = 0;
-      if (j0 + j < end && sees(j0 + j)) e = exp_fixed((((int64_t)score(j0 + j) - (int64_t)mx) * ONE) >> 14);
-      if (lane == 0) {
-        es[j] = (int32_t)e;
-        atomicAdd(&ssum, (unsigned long long)e);
+#pragma unroll 1
+    for (int t = warp; t < nt; t += NW) {
+      const int32_t *kn = row_of(min(t + NW, nt - 1));
+      int32_t acc[MT][7][4];
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int c = 0; c < 7; c++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[m][c][i] = 0;
+#pragma unroll
+      for (int k0 = 0; k0 < KS; k0 += KG) {
+        uint32_t k3 = 0u;
+#pragma unroll
+        for (int i = 0; i < KG; i++) {
+          uint32_t b0[4], b1[4];
+          digits(kb[i][0].x, kb[i][0].y, kb[i][0].z, kb[i][0].w, b0);
+          digits(kb[i][1].x, kb[i][1].y, kb[i][1].z, kb[i][1].w, b1);
+          k3 |= b0[3] | b1[3];
+#pragma unroll
+          for (int p = 0; p < 3; p++)
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+              const uint4 A = qf[((m * KS + k0 + i) * 4 + p) * 32 + lane];
+#pragma unroll
+              for (int j = 0; j < 3; j++) mma_su(acc[m][p + j], A, b0[j], b1[j]);
+            }
+        }
+        if (__any_sync(0xffffffffu, k3 != 0u) || q3) {   // fourth digits
+#pragma unroll 1
+          for (int i = 0; i < KG; i++) {
+            int4 v0 = kb[0][0], v1 = kb[0][1];
+#pragma unroll
+            for (int j = 1; j < KG; j++)
+              if (i == j) { v0 = kb[j][0]; v1 = kb[j][1]; }
+            uint32_t b0[4], b1[4];
+            digits(v0.x, v0.y, v0.z, v0.w, b0);
+            digits(v1.x, v1.y, v1.z, v1.w, b1);
+#pragma unroll
+            for (int m = 0; m < MT; m++) {
+#pragma unroll
+              for (int p = 0; p < 4; p++)
+                mma_ss(acc[m][p + 3], qf[((m * KS + k0 + i) * 4 + p) * 32 + lane], b0[3], b1[3]);
+              const uint4 A = qf[((m * KS + k0 + i) * 4 + 3) * 32 + lane];
+#pragma unroll
+              for (int j = 0; j < 3; j++) mma_su(acc[m][3 + j], A, b0[j], b1[j]);
+            }
+          }
+        }
+        load(k0 + KG < KS ? kr + (k0 + KG) * 32 : kn);
+      }
+      kr = kn;
+      const int slot = cb + t * 8 + 2 * c4;   // this lane's two slots
+      const bool all = cb + t * 8 >= clear && cb + t * 8 + 8 <= min(q.ctx, c1);
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const int x = m * 16 + n8 + h * 8;
+          const int64_t off = -BIAS * (int64_t)qsum[x];
+          int32_t z[2];
+          bool see[2] = {true, true};
+          if (!all) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+              const int sl = slot + i;
+              see[i] = (sl < q.ctx ? sl >= first[x] : ((seen[x] >> ((sl - q.ctx) & 63)) & 1ull) != 0) && sl < c1;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 2; i++) {
+            const int e = 2 * h + i;
+            int64_t s = off + acc[m][0][e];
+            s += (int64_t)acc[m][1][e] * 256;
+            s += (int64_t)acc[m][2][e] * 65536;
+            s += (int64_t)acc[m][3][e] * 16777216;
+            s += (int64_t)(acc[m][4][e] + acc[m][5][e] * 256 + acc[m][6][e] * 65536) << 32;
+            // f32 of the score (one rounding: below 2^53 wherever |z| < 2^17), then z 2^14 rounded half
+            // away from zero: adding a half towards zero never crosses a whole number
+            float v = __fmul_rn(__ll2float_rn(s), scale);
+            if (!(fabsf(v) < 2147483648.0f)) {
+              if (see[i]) raise_err(a.err, ERR_SCORE_RANGE);
+              v = 0.0f;
+            }
+            z[i] = see[i] ? __float2int_rz(__fadd_rz(v, copysignf(0.5f, v))) : UNSEEN;
+            lmax[m][h] = max(lmax[m][h], z[i]);
+          }
+          *reinterpret_cast<int2 *>(sc + x * SCS + t * 8 + 2 * c4) = make_int2(z[0], z[1]);
+        }
+    }
+    if (want_max) {
+#pragma unroll
+      for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          int32_t v = lmax[m][h];
+          v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
+          v = max(v, __shfl_xor_sync(0xffffffffu, v, 2));
+          if (c4 == 0 && v != UNSEEN) atomicMax(&mx[m * 16 + n8 + h * 8], v);
+        }
+    }
+    __syncthreads();
+  };
+
+  // ---- exponentials in place: four neighbours' scores become their bytes' planes
+  auto exps = [&](int len) {
+    for (int x = warp; x < QV; x += NW) {
+      const int32_t m = mx[x];
+      int64_t sum = 0;
+      for (int i = lane; i < ((len + 31) & ~31) / 4; i += 32) {
+        int4 *p = reinterpret_cast<int4 *>(sc + x * SCS) + i;
+        const int4 z = *p;
+        const uint32_t e0 = exp_grid(z.x, m), e1 = exp_grid(z.y, m), e2 = exp_grid(z.z, m), e3 = exp_grid(z.w, m);
+        sum += (int64_t)e0 + e1 + (int64_t)e2 + e3;
+        *reinterpret_cast<uint4 *>(p) = bytes4(e0, e1, e2, e3);
+      }
+      sum = warp_sum_i64(sum);
+      if (lane == 0) ssum[x] += sum;
+    }
+    __syncthreads();
+  };
+
+  // ---- V-sums: warp (dg, pg) takes dims dg 8 ND .. of the pass over every PG-th run of 32 slots
+  const int dg = warp % T::DG, pg = warp / T::DG;
+  int32_t acc[MT][ND][7][4];
+  int32_t vv[2][4][ND];   // a run's V rows, on their way while the run before is multiplied
+  auto vload = [&](int st, int nst, int d0) {
+    const int32_t *vb = q.kv.v + d0 + dg * 8 * ND + ND * n8;
+    st = min(st, nst - 1);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint4 r = *reinterpret_cast<const uint4 *>(rows + st * 32 + h * 16 + 4 * c4);
+      ld_kv<ND>(vv[h][0], vb + (size_t)r.x * HD);
+      ld_kv<ND>(vv[h][1], vb + (size_t)r.y * HD);
+      ld_kv<ND>(vv[h][2], vb + (size_t)r.z * HD);
+      ld_kv<ND>(vv[h][3], vb + (size_t)r.w * HD);
+    }
+  };
+  auto vsums = [&](int len, int d0) {   // (the first run's rows are on their way)
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int c = 0; c < 7; c++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[m][d][c][i] = 0;
+    const int nst = (len + 31) / 32;
+#pragma unroll 1
+    for (int st = pg; st < nst; st += T::PG) {
+      uint32_t b[ND][2][4], v3 = 0u;   // [dim][half][plane]
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          digits(vv[h][0][d], vv[h][1][d], vv[h][2][d], vv[h][3][d], b[d][h]);
+          v3 |= b[d][h][3];
+        }
+      vload(st + T::PG, nst, d0);
+      const bool any3 = __any_sync(0xffffffffu, v3 != 0u);
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        const uint32_t *e = reinterpret_cast<const uint32_t *>(sc) + (m * 16 + n8) * SCS + st * 32 + 4 * c4;
+        const uint4 r0 = *reinterpret_cast<const uint4 *>(e), r1 = *reinterpret_cast<const uint4 *>(e + 8 * SCS);
+        const uint4 r2 = *reinterpret_cast<const uint4 *>(e + 16), r3 = *reinterpret_cast<const uint4 *>(e + 8 * SCS + 16);
+        const uint4 A[4] = {make_uint4(r0.x, r1.x, r2.x, r3.x), make_uint4(r0.y, r1.y, r2.y, r3.y),
+                            make_uint4(r0.z, r1.z, r2.z, r3.z), make_uint4(r0.w, r1.w, r2.w, r3.w)};
+#pragma unroll
+        for (int p = 0; p < 4; p++)
+#pragma unroll
+          for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int j = 0; j < 3; j++) mma_uu(acc[m][d][p + j], A[p], b[d][0][j], b[d][1][j]);
+        if (any3) {
+#pragma unroll
+          for (int p = 0; p < 4; p++)
+#pragma unroll
+            for (int d = 0; d < ND; d++) mma_us(acc[m][d][p + 3], A[p], b[d][0][3], b[d][1][3]);
+        }
       }
     }
-    __syncthreads();
-    if (tid < HD)
-      for (int j = 0; j < min(TT, end - j0); j++)
-        if (es[j]) acc128_add(acc, (int64_t)es[j] * q.kv.v[tree_row(a.c, q.kv, a.layer, g, j0 + j, a.err) + tid]);
+  };
+  // V-sum = lo + hi 2^32: four classes below 2^31 each fit lo with room for every rank's, three fit hi
+  auto fold = [&](int m, int d, int i) {
+    const int32_t(&c)[7][4] = acc[m][d];
+    longlong2 r;
+    r.x = c[0][i] + (long long)c[1][i] * 256 + (long long)c[2][i] * 65536 + (long long)c[3][i] * 16777216;
+    r.y = c[4][i] + (long long)c[5][i] * 256 + (long long)c[6][i] * 65536;
+    return r;
+  };
+  auto each = [&](auto &&f) {   // (query vector, dim inside the pass, V-sum) of this lane's accumulators
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) f(m * 16 + n8 + (i >> 1) * 8, dg * 8 * ND + ND * (2 * c4 + (i & 1)) + d, fold(m, d, i));
+  };
+
+  if (!MULTI) {   // (the launch gave every rank CS slots at most)
+    if (c0 < c1) locate(c0, c1 - c0);
+    scores(c0, c1 - c0, true);
+    if (c0 < c1) vload(pg, (c1 - c0 + 31) / 32, 0);   // across the exchange and the exponentials
+  } else {
+    for (int cb = c0; cb < c1; cb += CS) {
+      locate(cb, min(CS, c1 - cb));
+      scores(cb, min(CS, c1 - cb), true);
+    }
+  }
+  if (CL > 1) {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // every rank has started
+    for (int i = tid; i < CL * QV; i += TT) *cluster.map_shared_rank(&mx_in[rank][i % QV], i / QV) = mx[i % QV];
+    cluster.sync();
+    if (tid < QV) {
+      int32_t m = UNSEEN;
+      for (int r = 0; r < CL; r++) m = max(m, mx_in[r][tid]);
+      mx[tid] = m;
+    }
     __syncthreads();
   }
-  if (tid < HD) {
-    const int64_t hi = (int64_t)(((uint64_t)acc.hi << 16) | (acc.lo >> 48));
-    const int64_t qd = floordiv_s128(hi, acc.lo << 16, ssum);
-    const float o = __double2float_rn(__dmul_rn(__ll2double_rn(qd), 0x1p-32));
-    a.out[((size_t)row * a.NH + h) * HD + tid] = o;
-    if (a.ao_max) atomicMax(a.ao_max + row, __float_as_uint(fabsf(o)));
+  if (MULTI) {
+    for (int i = tid; i < QV * HD; i += TT) keep[i] = make_longlong2(0, 0);
+    for (int cb = c0; cb < c1; cb += CS) {
+      const int len = min(CS, c1 - cb);
+      __syncthreads();
+      locate(cb, len);
+      scores(cb, len, false);
+      exps(len);
+#pragma unroll 1
+      for (int ps = 0; ps < T::PASSES; ps++) {
+        vload(pg, (len + 31) / 32, ps * T::DP);
+        vsums(len, ps * T::DP);
+        for (int r = 0; r < T::PG; r++) {   // (the slot groups add to the same sums in turn)
+          if (pg == r)
+            each([&](int x, int d, longlong2 v) {
+              longlong2 &k = keep[x * HD + ps * T::DP + d];
+              k.x += v.x;
+              k.y += v.y;
+            });
+          if (T::PG > 1) __syncthreads();
+        }
+      }
+    }
+  } else {
+    exps(c1 - c0);
+#pragma unroll 1
+    for (int ps = 0; ps < T::PASSES; ps++) {
+      if (ps > 0 && c0 < c1) vload(pg, (c1 - c0 + 31) / 32, ps * T::DP);
+      vsums(c1 - c0, ps * T::DP);
+      if (ps + 1 < T::PASSES) each([&](int x, int d, longlong2 v) { keep[(ps * QV + x) * T::DP + d] = v; });
+    }
+  }
+  // ---- join: dim d's sums go to rank d / DPR; the last pass straight from registers
+  if (CL > 1) cluster.sync();   // every rank is done with its scores: their memory takes the sums
+  else __syncthreads();
+  const int DPR = HD / CL, lg = 31 - __clz(DPR), src = MULTI ? 1 : T::PG;   // (a power of two; sums per rank)
+  auto push = [&](int x, int d, longlong2 v) {
+    longlong2 *to = sums + ((((rank * src + (MULTI ? 0 : pg)) * QV + x) << lg) | (d & (DPR - 1)));
+    if (CL > 1) to = cluster.map_shared_rank(to, d >> lg);
+    *to = v;
+  };
+  if (MULTI) {
+    for (int i = tid; i < QV * HD; i += TT) push(i / HD, i % HD, keep[i]);
+  } else {
+    each([&](int x, int d, longlong2 v) { push(x, (T::PASSES - 1) * T::DP + d, v); });
+    for (int i = tid; i < (T::PASSES - 1) * QV * T::DP; i += TT) {   // (PG is 1 with passes)
+      const int ps = i / (QV * T::DP), r = i % (QV * T::DP);
+      push(r / T::DP, ps * T::DP + r % T::DP, keep[i]);
+    }
+  }
+  static_assert(T::PASSES == 1 || T::PG == 1, "one slot group where there are passes");
+  if (CL > 1) {
+    for (int i = tid; i < CL * QV; i += TT) *cluster.map_shared_rank(&s_in[rank][i % QV], i / QV) = ssum[i % QV];
+    cluster.sync();   // the last cluster access
+    if (tid < QV) {
+      long long s = 0;
+      for (int r = 0; r < CL; r++) s += s_in[r][tid];
+      ssum[tid] = s;
+    }
+  }
+  if (tid < QV) rinv[tid] = __ddiv_rn(65536.0, __ll2double_rn(ssum[tid]));
+  __syncthreads();
+  for (int i = tid; i < nq << lg; i += TT) {
+    const int x = i >> lg, d = i & (DPR - 1), node = (x0 + x) / G, h = (x0 + x) % G;
+    long long lo = 0, hi = 0;
+    for (int r = 0; r < CL * src; r++) {
+      const longlong2 v = sums[((r * QV + x) << lg) | d];
+      lo += v.x;
+      hi += v.y;
+    }
+    const long long S = ssum[x];
+    acc128 N{0ull, 0ll};   // lo + hi 2^32 - BIAS sum e
+    acc128_add(N, lo);
+    acc128_add(N, acc128{(uint64_t)hi << 32, hi >> 32});
+    acc128_add(N, acc128{(uint64_t)(-BIAS * S), __mul64hi(-BIAS, S)});
+    const float o = finish(N, (uint64_t)S, rinv[x]);
+    a.out[((size_t)(q.row0 + node) * a.NH + (size_t)g * G + h) * HD + rank * DPR + d] = o;
+    if (a.ao_max) atomicMax(&omx[node - x0 / G], __float_as_uint(fabsf(o)));   // (a tile may begin inside a node's heads)
+  }
+  if (a.ao_max) {
+    __syncthreads();
+    if (tid < QV && omx[tid]) atomicMax(a.ao_max + q.row0 + x0 / G + tid, omx[tid]);
   }
 }
 
@@ -206,8 +735,8 @@ bool tree_pdl() {
   return on;
 }
 
-template <typename A>
-cudaError_t launch(void (*kern)(A), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, const A &a) {
+template <typename... K, typename... A>
+cudaError_t launch(void (*kern)(K...), dim3 grid, dim3 block, size_t smem, int cluster, cudaStream_t st, const A &...a) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
@@ -229,14 +758,92 @@ cudaError_t launch(void (*kern)(A), dim3 grid, dim3 block, size_t smem, int clus
   }
   cfg.attrs = attr;
   cfg.numAttrs = na;
-  return cudaLaunchKernelEx(&cfg, kern, a);
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<K>(a)...);
+}
+
+}  // namespace
+
+namespace {
+
+// Slots that a CTA's fixed work (finding its tile, the queries, three cluster barriers, the join) costs
+// as much time as.
+constexpr int TREE_FIXED = 256;
+
+template <int HD, int MT, bool MULTI>
+cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, int span, cudaStream_t st) {
+  using T = TreeTile<HD, MT, MULTI>;
+  auto kern = k_tree_attn<HD, MT, MULTI>;
+  // CTAs that run at once, by cluster size (asked once per device, before any launch: a capture never
+  // sees a failed launch)
+  static int room[64][5];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  dev &= 63;
+  if (room[dev][0] == 0) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    for (int i = 4; i >= 0; i--) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1 << i);
+      cfg.blockDim = dim3(T::TT);
+      cfg.dynamicSmemBytes = T::SMEM;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1 << i;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
+      room[dev][i] = n << i;
+    }
+    (void)cudaGetLastError();
+    if (room[dev][0] <= 0) return cudaErrorLaunchOutOfResources;
+  }
+  // the cluster size whose waves of CTAs take the least slots one after the other
+  int best = -1;
+  long long cost = 0;
+  for (int i = 0; i < 5; i++) {
+    const long long per = ((span + (1 << i) - 1) / (1 << i) + 31) & ~31;
+    if (room[dev][i] <= 0 || (!MULTI && per > T::CS)) continue;
+    const long long waves = ((tiles * a.c.NKV << i) + room[dev][i] - 1) / room[dev][i];
+    const long long c = waves * (per + TREE_FIXED);
+    if (best < 0 || c < cost) { best = i; cost = c; }
+  }
+  if (best < 0) return cudaErrorInvalidValue;
+  return launch(kern, dim3(1 << best, a.c.NKV, (unsigned)tiles), dim3(T::TT), T::SMEM, 1 << best, st, a, 1 << best);
+}
+
+template <int HD>
+cudaError_t tree_attn_hd(const TreeAttnArgs &a, cudaStream_t st) {
+  const int G = a.NH / a.c.NKV;
+  // two row tiles per CTA where a sequence's queries fill them; more slots than a cluster of 16 keeps
+  // scores for go in runs
+  const int span = (a.win >= 0 && a.win < a.max_ctx ? a.win : a.max_ctx) + TREE_NODES;
+  const bool multi = span > 16 * TreeTile<HD, 1, false>::CS;
+  const bool two = !multi && (long long)a.c.rows * G > 16ll * a.c.n_seq;
+  const int QV = two ? 32 : 16;
+  // tiles: every sequence's last one may be partly filled
+  const long long most = (long long)a.c.n_seq * ((TREE_NODES * G + QV - 1) / QV);
+  long long tiles = a.c.n_seq == 1 ? ((long long)a.c.rows * G + QV - 1) / QV : (long long)a.c.rows * G / QV + a.c.n_seq;
+  if (tiles > most) tiles = most;
+  if (tiles > 65535) return cudaErrorInvalidValue;
+  if (multi) return tree_attn<HD, 1, true>(a, tiles, span, st);
+  return two ? tree_attn<HD, 2, false>(a, tiles, span, st) : tree_attn<HD, 1, false>(a, tiles, span, st);
 }
 
 }  // namespace
 
 cudaError_t launch_tree_attn(const TreeAttnArgs &a, cudaStream_t st) {
   if (a.c.rows <= 0) return cudaSuccess;
-  return launch(k_tree_attn, dim3(a.NH, a.c.rows), dim3(TT), 0, 1, st, a);
+  switch (a.c.HD) {
+    case 64: return tree_attn_hd<64>(a, st);
+    case 128: return tree_attn_hd<128>(a, st);
+    case 256: return tree_attn_hd<256>(a, st);
+  }
+  return cudaErrorInvalidValue;
 }
 
 cudaError_t launch_kv_compact(const KvCompactArgs &a, cudaStream_t st) {

@@ -10,6 +10,7 @@
 namespace spb {
 
 constexpr int TREE_NODES = 64;   // drafted tokens of one sequence: an ancestor set is one 64-bit word
+constexpr int TREE_SPAN = 1 << 20; // slots a node may see: the V-sums' low words stay below 2^63
 
 // One sequence: its cache, the positions it holds, its rows [row0, row0 + n) among the step's
 // (node i cached in slot ctx + i) and the slots its page table reaches.

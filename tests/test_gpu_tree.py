@@ -154,7 +154,7 @@ def test_attention_is_the_contract(cuda_ok, NKV, G, HD, page, ctx, nodes, win):
     assert np.array_equal(u32(got), u32(c.want(win)))
 
 
-@pytest.mark.parametrize("HD,G,ctx,nodes", [(64, 2, 1500, 6), (256, 2, 700, 20), (128, 4, 2600, 3)])
+@pytest.mark.parametrize("HD,G,ctx,nodes", [(64, 2, 1500, 6), (256, 2, 700, 20), (128, 4, 2600, 3), (64, 2, 18000, 3), (256, 1, 17500, 2)])
 def test_attention_long_contexts(cuda_ok, HD, G, ctx, nodes):
     c = Case(3, 1, G, HD, 128, [ctx], [tree(np.random.default_rng(1), nodes, 0.7)]).upload()
     assert np.array_equal(u32(c.run().cpu().numpy()), u32(c.want()))

@@ -29,7 +29,7 @@ BAD, UNS = spb200.SPB_EBADARG, spb200.SPB_EUNSUPPORTED
 @pytest.mark.parametrize("kw,code", [
     (dict(k=None), BAD), (dict(v=None), BAD), (dict(n_pages=0), BAD), (dict(page=0), BAD), (dict(page=-8), BAD), (dict(ptab_ld=0), BAD),
     (dict(n_layers=0), BAD), (dict(n_head_kv=0), BAD), (dict(head_dim=96), UNS), (dict(head_dim=32), UNS),
-    (dict(k=260), BAD), (dict(v=264), BAD), (dict(ptab=None, n_pages=1), BAD),
+    (dict(k=260), BAD), (dict(v=272), BAD), (dict(ptab=None, n_pages=1), BAD),
 ])
 def test_cache_views_are_checked(kw, code):
     v = view(**kw)
