@@ -278,8 +278,8 @@ int spb_kv_compact(const spb_kv_view *kv, int n_seq, const int32_t *ctx, const i
  * and gives NaN), lse and entropy [rows] (each NULL: not wanted), and the top (0..32) largest entries'
  * ids and log probabilities, equal entries lowest id first. -inf entries are masked tokens: logprob
  * -inf, no alternative (id -1, -inf where a row has fewer than top). A row of -inf alone has lse -inf
- * and entropy 0; a row with NaN or +inf has no distribution: NaN, ids -1. A row's results do not depend
- * on the other rows of the call. Device buffers of the current device; no workspace. */
+ * and entropy 0; a row with NaN or +inf has no distribution: NaN, ids -1. A row's bytes depend neither on
+ * the other rows of the call nor on its alignment. vocab at most 4194304 (SPB_EUNSUPPORTED). Device buffers of the current device; no workspace. */
 int spb_logprobs(const float *logits, int rows, int vocab, int64_t ld, const int32_t *tok_row,
                  const int32_t *tok, int n_tok, float *logprob, float *lse, float *entropy, int top,
                  int32_t *top_id, float *top_logprob, void *stream);

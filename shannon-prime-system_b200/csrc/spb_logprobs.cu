@@ -5,105 +5,383 @@
 // with m the row's maximum. -inf entries are masked tokens and weigh nothing. A row without a
 // finite or +inf entry has lse -inf and entropy 0; a row that holds NaN or +inf has no
 // distribution: lse, entropy, its tokens' logprobs and its alternatives' are NaN, the ids -1.
+//
+// One pass over the logits, so memory bounds it. A row is cut into up to 16 parts of at least 16384 entries;
+// a CTA's thread takes every 512th group of four neighbours of a part, a warp joins its threads' sums, and a
+// part its sixteen warps'. A cluster of C CTAs shares the parts of a row; C follows from the rows of the
+// call (few rows: a row over many CTAs), but what is summed in which order follows from the vocabulary's
+// size alone, so a row's bytes depend neither on the other rows nor on its alignment.
+//
+// A thread sums e^(x - m) = 2^(x L - M), L = log2(e) in f32 and M = m L rounded, for a reference m that is
+// its first groups' maximum and moves only when entries are more than 2^RISE above it; the weighted sum
+// takes the same exponents. L's rounding scales every entry by 1 + 1.3e-8, M's is taken off at the end.
+//
+// The largest entries: the top'th largest of the threads' maxima bounds the top'th largest entry from below,
+// and only the threads that reach it can hold larger ones: their groups are read again (from L2) and what
+// reaches the bound is ranked by counting. Rows whose large entries crowd into few threads' groups, or are
+// equal in great number, can overflow that list: they find one entry after the other.
+#include <cooperative_groups.h>
+#include <cstdlib>
+
 #include "spb_exact.cuh"
 #include "spb_tree.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace spb {
 
 namespace {
 
-constexpr int LT = 256;
+constexpr int LT = 512, LW = LT / 32;
+constexpr int LPART = 16384;       // entries of a part, up to 16 parts
+constexpr int LPARTS = 16;
+constexpr int LCAND = 2048;        // entries at or above the bound that are ranked by counting
+constexpr int LBATCH = 4;          // groups of four in flight per thread
+constexpr float LOG2E_F = 1.44269504f;
+constexpr float FLOOR2 = -200.0f;  // exponents of two below this are zero in f32
+constexpr float RISE = 16.0f;      // entries this far above the reference move it (e^16 times 2^22 entries fit f32)
 
-// larger value first, equal values lowest id first (-0 and +0 are equal); 0 is below every entry
-__device__ __forceinline__ unsigned long long top_key(float v, int id) {
+// larger value first, equal values lowest id first (-0 and +0 are equal); every entry above -inf is above 0
+__device__ __forceinline__ uint32_t ordered(float v) {
   const uint32_t b = __float_as_uint(__fadd_rn(v, 0.0f));
-  const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-  return ((unsigned long long)o << 32) | (uint32_t)~id;
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long top_key(float v, int id) {
+  return v > -INFINITY ? ((unsigned long long)ordered(v) << 32) | (uint32_t)~id : 0ull;
+}
+__device__ __forceinline__ float key_value(unsigned long long k) {
+  const uint32_t o = (uint32_t)(k >> 32);
+  return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
 }
 
-__device__ float block_sum(float v, float *red) {
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+struct Running {
+  float m, s, t;   // reference, sum of 2^((x - m) L), the same weighted by its exponent
+  float top;       // largest entry
+};
+
+// part [p0, p1) of a row that starts SH floats behind a 16-byte boundary
+template <int SH, bool ENT>
+__device__ __forceinline__ void part(const float *x, int p0, int p1, int vocab, Running &r) {
+  const int lane = threadIdx.x & 31, b1 = (p1 + 3) >> 2;
+  const float4 *xa = reinterpret_cast<const float4 *>(x - SH);   // group b is entries 4 b .. of xa, SH on
+#pragma unroll 1
+  for (int b0 = (p0 >> 2) + (int)threadIdx.x - lane; b0 < b1; b0 += LBATCH * LT) {   // (warp-uniform)
+    float v[LBATCH][4];
+    const int last = b0 + (LBATCH - 1) * LT + 31;   // the batch's last group
+    if (last < b1 && 4 * last + (SH ? 8 : 4) <= vocab && (SH == 0 || b0 > 0)) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.0f;
-  for (int i = 0; i < LT / 32; i++) s += red[i];
-  return s;
+      for (int u = 0; u < LBATCH; u++) {
+        const int b = b0 + u * LT + lane;
+        const float4 c = xa[b];
+        v[u][0] = c.x; v[u][1] = c.y; v[u][2] = c.z; v[u][3] = c.w;
+        if (SH) {   // (the rest of the group: the neighbour's line, from L1)
+          const float4 d = xa[b + 1];
+          const float w[8] = {c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[u][i] = w[SH + i];
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < LBATCH; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int e = 4 * (b0 + u * LT + lane) + i;
+          v[u][i] = e < p1 ? x[e] : -INFINITY;
+        }
+    }
+    float bm = v[0][0];
+#pragma unroll
+    for (int u = 0; u < LBATCH; u++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) bm = fmaxf(bm, v[u][i]);
+    r.top = fmaxf(r.top, bm);
+    if (bm > __fadd_rn(r.m, RISE)) {   // (a first finite entry, or a steep rise)
+      const float a = fmaxf(__fmul_rn(__fsub_rn(r.m, bm), LOG2E_F), FLOOR2), f = exp2_fast(a);
+      r.t = __fmul_rn(f, __fmaf_rn(r.s, a, r.t));
+      r.s = __fmul_rn(r.s, f);
+      r.m = bm;
+    }
+    const float m = r.m == -INFINITY ? 0.0f : r.m, M = __fmul_rn(m, LOG2E_F);
+    if (fabsf(m) < 1e37f) {
+      float s = 0.0f, t = 0.0f;
+#pragma unroll
+      for (int u = 0; u < LBATCH; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float a = max_nan(__fmaf_rn(v[u][i], LOG2E_F, -M), FLOOR2), e = exp2_fast(a);
+          s = __fadd_rn(s, e);
+          if (ENT) t = __fmaf_rn(e, a, t);
+        }
+      const float d = __fmaf_rn(m, LOG2E_F, -M);   // M's rounding, exactly: 2^-d = 1 - d ln 2
+      r.t = __fadd_rn(r.t, __fmaf_rn(-d, __fmaf_rn(0.693147182f, t, s), t));
+      r.s = __fadd_rn(r.s, __fmaf_rn(__fmul_rn(-d, 0.693147182f), s, s));
+    } else {   // (m L may overflow)
+#pragma unroll
+      for (int u = 0; u < LBATCH; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float a = max_nan(__fmul_rn(__fsub_rn(v[u][i], m), LOG2E_F), FLOOR2), e = exp2_fast(a);
+          r.s = __fadd_rn(r.s, e);
+          r.t = __fmaf_rn(e, a, r.t);
+        }
+    }
+  }
 }
 
-__device__ unsigned long long block_max_u64(unsigned long long v, unsigned long long *red) {
+__device__ __forceinline__ unsigned long long warp_max_u64(unsigned long long v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  unsigned long long m = 0;
-  for (int i = 0; i < LT / 32; i++) m = max(m, red[i]);
-  return m;
+  return v;
 }
 
-// One CTA per row, one pass per quantity.
-__global__ void __launch_bounds__(LT) k_logprobs(LogprobArgs a) {
-  __shared__ float red[LT / 32];
-  __shared__ unsigned long long redk[LT / 32];
-  const int r = blockIdx.x, tid = threadIdx.x;
-  const float *x = a.x + (size_t)r * a.ld;
-  float m = -INFINITY;
-  bool bad = false;
-  for (int j = tid; j < a.vocab; j += LT) {
-    const float v = x[j];
-    bad |= !(v < INFINITY);
-    m = fmaxf(m, v);
+// (m, s, t) of two disjoint sets of entries as one, s and t being sums relative to m
+__device__ __forceinline__ void join(float &m, float &s, float &t, float m2, float s2, float t2) {
+  const float mm = fmaxf(m, m2);
+  const float a = m == -INFINITY ? FLOOR2 : max_nan(__fmul_rn(__fsub_rn(m, mm), LOG2E_F), FLOOR2);
+  const float b = m2 == -INFINITY ? FLOOR2 : max_nan(__fmul_rn(__fsub_rn(m2, mm), LOG2E_F), FLOOR2);
+  const float f = exp2_fast(a), g = exp2_fast(b);
+  t = __fadd_rn(__fmul_rn(f, __fmaf_rn(s, a, t)), __fmul_rn(g, __fmaf_rn(s2, b, t2)));
+  s = __fadd_rn(__fmul_rn(s, f), __fmul_rn(s2, g));
+  m = mm;
+}
+// over W neighbouring lanes (a power of two); every one of them gets the result
+template <int W>
+__device__ __forceinline__ void join_lanes(float &m, float &s, float &t) {
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
+    const float t2 = __shfl_xor_sync(0xffffffffu, t, o);
+    // (the same operands in the same order on both sides of the pair)
+    if ((threadIdx.x & o) == 0) join(m, s, t, m2, s2, t2);
+    else {
+      float mm = m2, ss = s2, tt = t2;
+      join(mm, ss, tt, m, s, t);
+      m = mm; s = ss; t = tt;
+    }
   }
-  bad = __syncthreads_or(bad);
-  unsigned long long k = block_max_u64(top_key(m, 0), redk);
-  {
-    const uint32_t o = (uint32_t)(k >> 32);
-    m = __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+}
+
+template <bool ENT>
+__global__ void __launch_bounds__(LT, 2) k_logprobs(LogprobArgs a, int C, int P, int per) {
+  __shared__ float um[LPARTS][LW], us[LPARTS][LW], ut[LPARTS][LW];   // this CTA's parts, warp by warp
+  __shared__ float pm[LPARTS], ps[LPARTS], pt[LPARTS];               // the row's parts, pushed by their ranks
+  __shared__ uint32_t list[LT], bound_sh, redv[LW];
+  __shared__ unsigned long long redk[LW], best[LOGPROB_TOP], cand[LCAND];
+  __shared__ unsigned long long in_best[16][LOGPROB_TOP];            // every rank's best, on rank 0
+  __shared__ int count, n_cand;
+  __shared__ float lse_sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = C > 1 ? (int)cluster.block_rank() : 0, row = blockIdx.x / C;
+  if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) { count = n_cand = 0; bound_sh = 1u; }
+  if (tid < LOGPROB_TOP) best[tid] = 0ull;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const float *x = a.x + (size_t)row * a.ld;
+  // this thread's first token of the call, if it is one of this row's, is on its way from the start
+  const int t0 = rank * LT + tid;
+  int tok0 = -1, row0 = -1;
+  float x0 = 0.0f;
+  if (t0 < a.n_tok) {
+    row0 = a.tok_row ? a.tok_row[t0] : t0;
+    tok0 = a.tok[t0];
+    if (row0 == row && tok0 >= 0 && tok0 < a.vocab) x0 = x[tok0];
   }
-  float s = 0.0f, t = 0.0f;
-  for (int j = tid; j < a.vocab; j += LT) {
-    const float d = x[j] - m, e = expf(d);
-    if (x[j] > -INFINITY) { s += e; t += e * d; }
+  // ---- the rank's parts: part p of every C
+  const int sh = (int)(((uintptr_t)x >> 2) & 3);
+  float largest = -INFINITY;   // this thread's
+#pragma unroll 1
+  for (int p = rank, i = 0; p < P; p += C, i++) {
+    const int p0 = p * per, p1 = min(p0 + per, a.vocab);
+    Running r{-INFINITY, 0.0f, 0.0f, -INFINITY};
+    switch (sh) {
+      case 0: part<0, ENT>(x, p0, p1, a.vocab, r); break;
+      case 1: part<1, ENT>(x, p0, p1, a.vocab, r); break;
+      case 2: part<2, ENT>(x, p0, p1, a.vocab, r); break;
+      default: part<3, ENT>(x, p0, p1, a.vocab, r); break;
+    }
+    largest = fmaxf(largest, r.top);
+    float m = r.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float d = r.m == -INFINITY ? FLOOR2 : max_nan(__fmul_rn(__fsub_rn(r.m, m), LOG2E_F), FLOOR2), f = exp2_fast(d);
+    float s = __fmul_rn(r.s, f), t = __fmul_rn(f, __fmaf_rn(r.s, d, r.t));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, o));
+      t = __fadd_rn(t, __shfl_xor_sync(0xffffffffu, t, o));
+    }
+    if (lane == 0) { um[i][warp] = m; us[i][warp] = s; ut[i][warp] = t; }
   }
-  s = block_sum(s, red);
-  t = block_sum(t, red);
-  float lse = m + logf(s), ent = logf(s) - t / s;
-  if (m == -INFINITY) { lse = -INFINITY; ent = 0.0f; }
-  if (bad) lse = ent = NAN;
-  if (tid == 0) {
-    if (a.lse) a.lse[r] = lse;
-    if (a.entropy) a.entropy[r] = ent;
+  // with alternatives: the ceil(top / 16)'th largest of the warp's maxima (top <= 32: one of the first two)
+  uint32_t key = 0u;
+  if (a.top > 0) {
+    key = largest > -INFINITY ? ordered(largest) : 0u;
+    uint32_t k1 = __reduce_max_sync(0xffffffffu, key);
+    if (a.top > LW) {
+      const int l = __ffs(__ballot_sync(0xffffffffu, key == k1)) - 1;
+      k1 = __reduce_max_sync(0xffffffffu, lane == l ? 0u : key);
+    }
+    if (lane == 0) redv[warp] = k1;
   }
-  for (int i = tid; i < a.n_tok; i += LT) {
-    const int tr = a.tok_row ? a.tok_row[i] : i;
+  __syncthreads();
+  if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");   // every rank has started
+  // warp i joins part i's warps and hands the part to every rank
+  if (rank + warp * C < P) {
+    float m = um[warp][lane & (LW - 1)], s = us[warp][lane & (LW - 1)], t = ut[warp][lane & (LW - 1)];
+    join_lanes<LW>(m, s, t);
+    const int p = rank + warp * C;
+    if (lane < C) {
+      if (C > 1) {
+        *cluster.map_shared_rank(&pm[p], lane) = m;
+        *cluster.map_shared_rank(&ps[p], lane) = s;
+        *cluster.map_shared_rank(&pt[p], lane) = t;
+      } else {
+        pm[p] = m; ps[p] = s; pt[p] = t;
+      }
+    }
+  }
+  if (a.top > 0) {
+    // at least `top` threads' maxima reach this: those go into a list, its top'th is the bound (fewer than
+    // `top` threads hold any entry above -inf: the bound is 1, every such entry counts)
+    uint32_t loose = redv[0];
+#pragma unroll
+    for (int w = 1; w < LW; w++) loose = min(loose, redv[w]);
+    if (key >= loose && key != 0u) list[atomicAdd(&count, 1)] = key;
+    __syncthreads();
+    const int n = count;
+    if (tid < n) {
+      const uint32_t k = list[tid];
+      int above = 0;
+      for (int i = 0; i < n; i++) above += list[i] > k || (list[i] == k && i < tid);
+      if (above == a.top - 1) bound_sh = k;
+    }
+    __syncthreads();
+    const uint32_t bound = bound_sh;
+    // the threads that reach the bound: their groups, by the whole warp
+    uint32_t win = __ballot_sync(0xffffffffu, key >= bound);
+    const int steps = (per + 4 * LT - 1) / (4 * LT), mine = (P - rank + C - 1) / C;
+    while (win) {
+      const int l = __ffs(win) - 1;
+      win &= win - 1;
+      for (int i = lane; i < 4 * steps * mine; i += 32) {
+        const int st = (i >> 2) % steps, p = rank + (i >> 2) / steps * C;
+        const int e = p * per + 4 * (warp * 32 + l + st * LT) + (i & 3);
+        if (e < min((p + 1) * per, a.vocab)) {
+          const unsigned long long k = top_key(x[e], e);
+          if ((uint32_t)(k >> 32) >= bound) {
+            const int at = atomicAdd(&n_cand, 1);
+            if (at < LCAND) cand[at] = k;
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const int nc = n_cand;
+    if (nc <= LCAND) {
+      for (int c = tid; c < nc; c += LT) {
+        const unsigned long long k = cand[c];
+        int above = 0;
+        for (int i = 0; i < nc; i++) above += cand[i] > k;
+        if (above < a.top) best[above] = k;
+      }
+    } else {   // one entry after the other
+      unsigned long long last = ~0ull;
+      for (int i = 0; i < a.top; i++) {
+        unsigned long long b = 0ull;
+        for (int p = rank; p < P; p += C)
+          for (int e = p * per + tid; e < min((p + 1) * per, a.vocab); e += LT) {
+            const unsigned long long k = top_key(x[e], e);
+            if (k < last && k > b) b = k;
+          }
+        b = warp_max_u64(b);
+        if (lane == 0) redk[warp] = b;
+        __syncthreads();
+        for (int w = 0; w < LW; w++) b = max(b, redk[w]);
+        __syncthreads();
+        last = b;
+        if (tid == 0) best[i] = b;
+      }
+    }
+    __syncthreads();
+    if (tid < a.top) {
+      if (C > 1) *cluster.map_shared_rank(&in_best[rank][tid], 0) = best[tid];
+      else in_best[0][tid] = best[tid];
+    }
+  }
+  if (C > 1) cluster.sync();   // the last cluster access
+  else __syncthreads();
+  // ---- every rank: the row's statistics
+  if (warp == 0) {
+    float m = -INFINITY, s = 0.0f, t = 0.0f;
+    if (lane < P) { m = pm[lane]; s = ps[lane]; t = pt[lane]; }
+    join_lanes<32>(m, s, t);
+    float lse = -INFINITY, ent = 0.0f;
+    if (!(s == s) || m == INFINITY) {
+      lse = ent = NAN;
+    } else if (s > 0.0f) {
+      lse = __fadd_rn(m, logf(s));
+      ent = __fsub_rn(logf(s), __fmul_rn(0.693147182f, __fdiv_rn(t, s)));
+    }
+    if (lane == 0) {
+      lse_sh = lse;
+      if (rank == 0) {
+        if (a.lse) a.lse[row] = lse;
+        if (a.entropy) a.entropy[row] = ent;
+      }
+    }
+  }
+  __syncthreads();
+  const float lse = lse_sh;
+  // ---- this row's tokens (row 0's cluster also reports the rows that are out of range)
+  for (int i = t0; i < a.n_tok; i += C * LT) {
+    const int tr = i == t0 ? row0 : a.tok_row ? a.tok_row[i] : i;
     if (tr < 0 || tr >= a.rows) {
-      if (r == 0) { raise_err(a.err, ERR_TOKEN); a.logprob[i] = NAN; }
+      if (row == 0) { raise_err(a.err, ERR_TOKEN); a.logprob[i] = NAN; }
       continue;
     }
-    if (tr != r) continue;
-    const int tok = a.tok[i];
+    if (tr != row) continue;
+    const int tok = i == t0 ? tok0 : a.tok[i];
     float v = NAN;
-    if (tok >= 0 && tok < a.vocab) v = bad ? NAN : x[tok] == -INFINITY ? -INFINITY : x[tok] - lse;
-    else if (tok != -1) raise_err(a.err, ERR_TOKEN);
+    if (tok >= 0 && tok < a.vocab) {
+      const float xv = i == t0 ? x0 : x[tok];
+      v = lse != lse ? NAN : xv == -INFINITY ? -INFINITY : __fsub_rn(xv, lse);
+    } else if (tok != -1) {
+      raise_err(a.err, ERR_TOKEN);
+    }
     a.logprob[i] = v;
   }
-  unsigned long long last = ~0ull;
-  for (int i = 0; i < a.top; i++) {
-    unsigned long long b = 0;
-    for (int j = tid; j < a.vocab; j += LT) {
-      const unsigned long long key = top_key(x[j], j);
-      if (x[j] > -INFINITY && key < last && key > b) b = key;
+  // ---- rank 0: the alternatives of all ranks
+  if (rank == 0 && a.top > 0) {
+    if (C > 1)
+      for (int i = tid; i < C * a.top; i += LT) {
+        const unsigned long long k = in_best[i / a.top][i % a.top];
+        if (k == 0ull) continue;
+        int above = 0;
+        for (int j = 0; j < C; j++)
+          for (int l = 0; l < a.top; l++) above += in_best[j][l] > k;
+        if (above < a.top) best[above] = k;   // (this rank's own have all been handed over)
+      }
+    __syncthreads();
+    if (tid < a.top) {
+      const unsigned long long k = best[tid];
+      const bool none = k == 0ull || lse != lse;
+      a.ids[(size_t)row * a.top + tid] = none ? -1 : (int)~(uint32_t)k;
+      a.best[(size_t)row * a.top + tid] = lse != lse ? NAN : none ? -INFINITY : __fsub_rn(key_value(k), lse);
     }
-    b = block_max_u64(b, redk);
-    last = b;
-    if (tid == 0) {
-      const int id = b && !bad ? (int)~(uint32_t)b : -1;
-      a.ids[(size_t)r * a.top + i] = id;
-      a.best[(size_t)r * a.top + i] = bad ? NAN : id < 0 ? -INFINITY : x[id] - lse;
-    }
-    if (!b) last = 0;
   }
 }
 
@@ -111,8 +389,49 @@ __global__ void __launch_bounds__(LT) k_logprobs(LogprobArgs a) {
 
 cudaError_t launch_logprobs(const LogprobArgs &a, cudaStream_t st) {
   if (a.rows <= 0) return cudaSuccess;
-  k_logprobs<<<a.rows, LT, 0, st>>>(a);
-  return cudaGetLastError();
+  int P = (a.vocab + LPART - 1) / LPART;
+  if (P > LPARTS) P = LPARTS;
+  const int per = ((a.vocab + P - 1) / P + 3) & ~3;
+  P = (a.vocab + per - 1) / per;
+  // few rows: a row over as many CTAs as it has parts; more: over fewer, so that the call is one wave of two
+  // CTAs per SM (64 rows x 262144, 20 alternatives: 45 us with at most one per SM, 29 with two, 43 and 61
+  // with two and four waves)
+  int C = P;
+  while (C > 1 && (long long)a.rows * C > 2 * 148) C = (C + 1) / 2;
+  static bool set[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (!set[dev & 63]) {
+    e = cudaFuncSetAttribute(k_logprobs<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    set[dev & 63] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(C * a.rows));
+  cfg.blockDim = dim3(LT);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int na = 0;
+  static const bool pdl = [] {
+    const char *v = getenv("SPB_PDL");
+    return !(v && v[0] == '0');
+  }();
+  if (pdl) {
+    attr[na].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[na].val.programmaticStreamSerializationAllowed = 1;
+    na++;
+  }
+  if (C > 1) {
+    attr[na].id = cudaLaunchAttributeClusterDimension;
+    attr[na].val.clusterDim.x = C;
+    attr[na].val.clusterDim.y = attr[na].val.clusterDim.z = 1;
+    na++;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = na;
+  return a.entropy ? cudaLaunchKernelEx(&cfg, k_logprobs<true>, a, C, P, per) : cudaLaunchKernelEx(&cfg, k_logprobs<false>, a, C, P, per);
 }
 
 }  // namespace spb

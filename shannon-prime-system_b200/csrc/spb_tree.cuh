@@ -51,7 +51,8 @@ struct KvCompactArgs {
 };
 cudaError_t launch_kv_compact(const KvCompactArgs &a, cudaStream_t st);
 
-constexpr int LOGPROB_TOP = 32;    // alternatives of a row at most
+constexpr int LOGPROB_TOP = 32;          // alternatives of a row at most
+constexpr int LOGPROB_VOCAB = 1 << 22;   // entries of a row at most
 
 struct LogprobArgs {
   const float *x;                  // [rows][ld]

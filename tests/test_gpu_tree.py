@@ -366,6 +366,8 @@ def lp_ref(x, tok_row, tok, top):
     for i, (r, t) in enumerate(zip(tok_row, tok)):
         if 0 <= r < len(x) and 0 <= t < x.shape[1] and not bad[r]:
             lp[i] = -np.inf if np.isneginf(x[r, t]) else x[r, t] - lse[r]
+    # differences below f32's lowest value (-3e38 - 3e38) have no f32 but -inf
+    lp[lp < -3.4028236e38], best[best < -3.4028236e38] = -np.inf, -np.inf
     return lp, lse, ent, ids, best
 
 
@@ -438,6 +440,35 @@ def test_logprobs_ties_and_order(cuda_ok):
                   -np.arange(V) / 1000.0, np.where(np.arange(V) == V - 1, 80.0, -80.0), np.where(np.arange(V) % 64 < 32, 3.0, 2.0),
                   (np.arange(V) % 4096 < 8) * 1.0]).astype(np.float32)
     check_lp(x, range(len(x)), [5] * len(x), 32)
+
+
+def test_logprobs_crowded_rows(cuda_ok):
+    """Large entries that crowd into few threads' groups, and great numbers of equal ones: the list of candidates
+    overflows. Few distinct values (as logits that came from 8 bits), whole rows of one value, -inf in between."""
+    V, r = 40003, np.random.default_rng(8)
+    x = np.tile(r.standard_normal(V).astype(np.float32), (310, 1))
+    x[:100, (np.arange(V) // 4) % 512 < 20] += 50.0
+    x[100:200] = np.rint(x[100:200] * 2)
+    x[200:300] = 1.25
+    x[300:] = np.where(np.arange(V) % 3 == 0, -np.inf, 2.0)
+    pick = [0, 99, 100, 200, 309]
+    got = run_lp(x, range(310), [7] * 310, 32)
+    want = lp_ref(x[pick], range(5), [7] * 5, 32)
+    tol, tol_e = lp_tol(x[pick], V)
+    for k, (g, w) in enumerate(zip(got, want)):
+        if k == 3:
+            assert np.array_equal(g[pick], w)
+        else:
+            near(g[pick], w, tol_e if k == 2 else tol)
+    assert np.array_equal(u32(got[4][0]), u32(got[4][50])) and np.array_equal(got[3][0], got[3][50])
+
+
+def test_logprobs_steep_rows(cuda_ok):
+    """Entries that rise by steps along the row (the running reference moves), and values near f32's ends."""
+    V = 70001
+    x = np.stack([np.linspace(-300, 300, V), np.linspace(300, -300, V), np.where(np.arange(V) == V - 1, 3e38, -3e38),
+                  np.full(V, -3.4e38), np.where(np.arange(V) % 1000 == 999, 1e37, 0.0), np.full(V, 2e37)]).astype(np.float32)
+    check_lp(x, range(len(x)), [V - 1] * len(x), 3)
 
 
 def test_logprobs_empty_and_broken_rows(cuda_ok):
