@@ -174,20 +174,21 @@ __device__ __forceinline__ void join_lanes(float &m, float &s, float &t) {
 }
 
 template <bool ENT>
-__global__ void __launch_bounds__(LT, 2) k_logprobs(LogprobArgs a, int C, int P, int per) {
+__global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P, int per) {
   __shared__ float um[LPARTS][LW], us[LPARTS][LW], ut[LPARTS][LW];   // this CTA's parts, warp by warp
   __shared__ float pm[LPARTS], ps[LPARTS], pt[LPARTS];               // the row's parts, pushed by their ranks
   __shared__ uint32_t list[LT], bound_sh, redv[LW];
   __shared__ unsigned long long redk[LW], best[LOGPROB_TOP], cand[LCAND];
   __shared__ unsigned long long in_best[16][LOGPROB_TOP];            // every rank's best, on rank 0
-  __shared__ int count, n_cand;
+  __shared__ int count, n_cand, n_win;
+  __shared__ uint16_t winner[LT];
   __shared__ float lse_sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = C > 1 ? (int)cluster.block_rank() : 0, row = blockIdx.x / C;
   if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (tid == 0) { count = n_cand = 0; bound_sh = 1u; }
+  if (tid == 0) { count = n_cand = n_win = 0; bound_sh = 1u; }
   if (tid < LOGPROB_TOP) best[tid] = 0ull;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float *x = a.x + (size_t)row * a.ld;
@@ -271,21 +272,30 @@ __global__ void __launch_bounds__(LT, 2) k_logprobs(LogprobArgs a, int C, int P,
     }
     __syncthreads();
     const uint32_t bound = bound_sh;
-    // the threads that reach the bound: their groups, by the whole warp
-    uint32_t win = __ballot_sync(0xffffffffu, key >= bound);
-    const int steps = (per + 4 * LT - 1) / (4 * LT), mine = (P - rank + C - 1) / C;
-    while (win) {
-      const int l = __ffs(win) - 1;
-      win &= win - 1;
-      for (int i = lane; i < 4 * steps * mine; i += 32) {
-        const int st = (i >> 2) % steps, p = rank + (i >> 2) / steps * C;
-        const int e = p * per + 4 * (warp * 32 + l + st * LT) + (i & 3);
-        if (e < min((p + 1) * per, a.vocab)) {
-          const unsigned long long k = top_key(x[e], e);
-          if ((uint32_t)(k >> 32) >= bound) {
-            const int at = atomicAdd(&n_cand, 1);
-            if (at < LCAND) cand[at] = k;
-          }
+    // the threads that reach the bound (`top` of them, more only where maxima are equal): their groups, an
+    // entry per thread
+    if (key >= bound && key != 0u) winner[atomicAdd(&n_win, 1)] = (uint16_t)tid;
+    __syncthreads();
+    const int steps = (per + 4 * LT - 1) / (4 * LT), mine = (P - rank + C - 1) / C, each = 4 * steps * mine;
+    const int entries = n_win * each;
+#pragma unroll 1
+    for (int i0 = tid; i0 < entries; i0 += 4 * LT) {
+      float v[4];
+      int id[4];
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int i = i0 + u * LT, w = i / each, j = i - w * each;
+        const int st = (j >> 2) % steps, p = rank + (j >> 2) / steps * C;
+        id[u] = i < entries ? p * per + 4 * (winner[w] + st * LT) + (j & 3) : a.vocab;
+        const bool in = i < entries && id[u] < min((p + 1) * per, a.vocab);
+        v[u] = in ? x[id[u]] : -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const unsigned long long k = top_key(v[u], id[u]);
+        if ((uint32_t)(k >> 32) >= bound) {
+          const int at = atomicAdd(&n_cand, 1);
+          if (at < LCAND) cand[at] = k;
         }
       }
     }
@@ -395,7 +405,7 @@ cudaError_t launch_logprobs(const LogprobArgs &a, cudaStream_t st) {
   P = (a.vocab + per - 1) / per;
   // few rows: a row over as many CTAs as it has parts; more: over fewer, so that the call is one wave of two
   // CTAs per SM (64 rows x 262144, 20 alternatives: 45 us with at most one per SM, 29 with two, 43 and 61
-  // with two and four waves)
+  // with two and four waves); many rows: a CTA each, three per SM
   int C = P;
   while (C > 1 && (long long)a.rows * C > 2 * 148) C = (C + 1) / 2;
   static bool set[64];
@@ -405,12 +415,18 @@ cudaError_t launch_logprobs(const LogprobArgs &a, cudaStream_t st) {
   if (!set[dev & 63]) {
     e = cudaFuncSetAttribute(k_logprobs<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 92 * 1024);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 92 * 1024);
     if (e != cudaSuccess) return e;
     set[dev & 63] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(C * a.rows));
   cfg.blockDim = dim3(LT);
+  // calls of one wave spread over all SMs: unused shared memory keeps a second (third) CTA off an SM, where
+  // the scheduler would fill it first (64 rows: 30 -> 26 us)
+  const long long ctas = (long long)a.rows * C;
+  cfg.dynamicSmemBytes = ctas <= 148 ? 92 * 1024 : ctas <= 2 * 148 ? 52 * 1024 : 0;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   int na = 0;
