@@ -109,11 +109,8 @@ __device__ __forceinline__ void ld_kv8(int4 &a, int4 &b, const int32_t *p) {
                : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
                : "l"(p));
 }
-template <int N>
-__device__ __forceinline__ void ld_kv(int32_t (&v)[N], const int32_t *p) {
-  static_assert(N == 1 || N == 2, "one or two columns");
-  if (N == 2) asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[N - 1]) : "l"(p));
-  else asm volatile("ld.global.b32 %0, [%1];" : "=r"(v[0]) : "l"(p));
+__device__ __forceinline__ void ld_kv2(int32_t (&v)[2], const int32_t *p) {
+  asm volatile("ld.global.v2.b32 {%0,%1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "l"(p));
 }
 
 constexpr int32_t UNSEEN = INT32_MIN;   // the score of a position that a node does not see
@@ -153,7 +150,7 @@ __device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
   return __double2float_rn(__dmul_rn(__ll2double_rn(floordiv_s128(hi, N.lo << 16, S)), 0x1p-32));
 }
 
-// One CTA: MT * 16 query vectors (a sequence's nodes x the G query heads of one KV head) over a run
+// One CTA: 16 query vectors (a sequence's nodes x the G query heads of one KV head) over a run
 // of slots; a cluster of CL CTAs covers the sequence's slots and joins maxima, sums and V-sums,
 // which are whole numbers, so no split changes a byte.
 //   scores    a warp takes 8 slots at a time: their K rows go from global memory straight into the
@@ -161,40 +158,37 @@ __device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
 //             are a byte transpose in registers), the queries' planes wait in shared memory
 //   exps      in place over the scores, each four neighbours' bytes transposed into the planes of
 //             the row operand
-//   V-sums    a warp takes 8 or 16 head dims over all slots of the run, V rows again straight from
-//             global memory (eight slots x one or two dims per lane and step)
+//   V-sums    a warp takes 16 head dims over the slots of the run, V rows again straight from global
+//             memory (eight slots x two dims per lane and step)
 // MULTI (more slots per rank than scores are kept for): the maxima first, then scores again in runs of
 // CS slots, each run's V-sums added up in shared memory.
-template <int HD, int MT, bool MULTI>
+template <int HD, bool MULTI>
 struct TreeTile {
-  static constexpr int QV = 16 * MT, KS = HD / 32;
+  static constexpr int QV = 16, KS = HD / 32;
   static constexpr int NW = 16, TT = 32 * NW;
-  static constexpr int ND = 2 / MT;                             // head dims of a lane's V rows: its 56 sums
-  static constexpr int DP = HD < 8 * ND * NW ? HD : 8 * ND * NW;   // head dims of one V pass
-  static constexpr int DG = DP / (8 * ND), PG = NW / DG;        // warps along them, groups along the slots
-  static constexpr int PASSES = HD / DP;
-  // slots whose scores are kept (their rows' stride is 16 words off a multiple of 32: no bank conflicts)
-  static constexpr int CS = MULTI ? 1056 : MT == 1 ? 2112 : 1088, SCS = CS + 16;
-  static constexpr size_t QF = (size_t)MT * KS * 4 * 512;       // the queries' planes
+  static constexpr int ND = 2;                                  // head dims of a lane's V rows: its 56 sums
+  static constexpr int DG = HD / (8 * ND), PG = NW / DG;        // warps along the dims, groups along the slots
+  // slots whose scores are kept, in blocks of 16 query vectors x 32 slots in the row operand's order:
+  // [slot half][row half][lane][4 slots], and then the exponentials' planes, [plane][lane][4 registers]
+  static constexpr int CS = MULTI ? 1056 : 2112;
+  static constexpr size_t QF = (size_t)KS * 4 * 512;            // the queries' planes
   static constexpr size_t SUMS = (size_t)QV * HD * 16;          // V-sums of a tile
-  // V-sums of the passes before the last (over the planes, not needed by then), or MULTI's running ones
-  static constexpr size_t KEEP = MULTI ? SUMS : (size_t)(PASSES - 1) * QV * DP * 16;
-  static constexpr size_t HEAD = MULTI ? KEEP + QF : (KEEP > QF ? KEEP : QF);
-  static constexpr size_t SC = (size_t)QV * SCS * 4;
+  static constexpr size_t HEAD = QF + (MULTI ? SUMS : 0);       // (MULTI: the running V-sums)
+  static constexpr size_t SC = (size_t)QV * CS * 4;
   static constexpr size_t WORK = SC + CS * 4;
   static constexpr size_t POST = SUMS * (MULTI ? 1 : PG);       // over the scores: every source's sums of this rank's dims
   static constexpr size_t SMEM = HEAD + (WORK > POST ? WORK : POST);
 };
 
-template <int HD, int MT, bool MULTI>
+template <int HD, bool MULTI>
 __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
-  using T = TreeTile<HD, MT, MULTI>;
-  constexpr int QV = T::QV, KS = T::KS, SCS = T::SCS, CS = T::CS, TT = T::TT, NW = T::NW, ND = T::ND;
-  constexpr int KG = KS < 4 ? KS : 4;                           // 32-column steps of K loaded at a time
+  using T = TreeTile<HD, MULTI>;
+  constexpr int QV = T::QV, KS = T::KS, CS = T::CS, TT = T::TT, NW = T::NW, ND = T::ND;
+  constexpr int KG = KS < 4 ? 1 : 2;                            // 32-column steps of K in one run of loads
   extern __shared__ __align__(128) uint8_t raw[];
-  longlong2 *keep = reinterpret_cast<longlong2 *>(raw);         // [QV][DP] per pass, MULTI: [QV][HD]
-  uint4 *qf = reinterpret_cast<uint4 *>(raw + (MULTI ? T::KEEP : 0));   // [MT][KS][4][32]
-  int32_t *sc = reinterpret_cast<int32_t *>(raw + T::HEAD);     // [QV][SCS]
+  uint4 *qf = reinterpret_cast<uint4 *>(raw);                   // [KS][4][32]
+  longlong2 *keep = reinterpret_cast<longlong2 *>(raw + T::QF); // MULTI: [QV][HD]
+  int32_t *sc = reinterpret_cast<int32_t *>(raw + T::HEAD);     // [CS / 32][512]
   uint32_t *rows = reinterpret_cast<uint32_t *>(raw + T::HEAD + T::SC);  // [CS] the slots' rows in K and V
   longlong2 *sums = reinterpret_cast<longlong2 *>(raw + T::HEAD);        // [CL][PG][QV][HD / CL]
   __shared__ int32_t par[TREE_NODES];
@@ -203,16 +197,16 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   __shared__ unsigned long long seen[QV];
   __shared__ int32_t bounds[2];                                 // the tile's first slot, its latest window start
   __shared__ int32_t mx[QV], mx_in[16][QV];
-  __shared__ long long ssum[QV], s_in[16][QV];
-  __shared__ unsigned long long qsum[QV];
+  __shared__ unsigned long long ssum[QV], s_in[16][QV], qsum[QV];
   __shared__ uint32_t omx[QV];
   __shared__ double rinv[QV];
+  __shared__ int32_t out_at[QV], node_of[QV];
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n8 = lane >> 2, c4 = lane & 3;
   const int rank = CL > 1 ? (int)cluster.block_rank() : 0, g = blockIdx.y;
   const int G = a.NH / a.c.NKV;
   pdl_trigger();
-  if (tid < QV) { mx[tid] = UNSEEN; ssum[tid] = 0; qsum[tid] = 0; omx[tid] = 0u; }
+  if (tid < QV) { mx[tid] = UNSEEN; ssum[tid] = qsum[tid] = 0ull; omx[tid] = 0u; }
   pdl_wait();
 
   // ---- which sequence: tiles are counted over the sequences in order (every warp for itself)
@@ -230,7 +224,7 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
       const int v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    const int z = (int)blockIdx.z - before - (incl - n);
+    const int z = (int)(blockIdx.x / CL) - before - (incl - n);
     const uint32_t hit = __ballot_sync(0xffffffffu, z >= 0 && z < n);
     if (hit) {
       const int l = __ffs(hit) - 1;
@@ -294,6 +288,8 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
     if (lane < QV) {
       first[lane] = f;
       seen[lane] = m;
+      node_of[lane] = (x0 + lane) / G - x0 / G;              // (a tile may begin inside a node's heads)
+      out_at[lane] = (q.row0 + (x0 + lane) / G) * a.NH + g * G + (x0 + lane) % G;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -305,12 +301,12 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   // ---- the other warps: the queries' digit planes in the row operand's order, and their sums
   bool top = false;
   if (warp > 0)
-    for (int i = tid - 32; i < MT * KS * 32; i += TT - 32) {
-      const int l = i & 31, ks = (i >> 5) % KS, mt = (i >> 5) / KS;
+    for (int i = tid - 32; i < KS * 32; i += TT - 32) {
+      const int l = i & 31, ks = i >> 5;
       uint32_t pl[4][4];
 #pragma unroll
       for (int u = 0; u < 4; u++) {   // (row, columns): the operand's four registers
-        const int x = mt * 16 + (l >> 2) + (u & 1) * 8, d = ks * 32 + (l & 3) * 8 + (u >> 1) * 4;
+        const int x = (l >> 2) + (u & 1) * 8, d = ks * 32 + (l & 3) * 8 + (u >> 1) * 4;
         int4 v = make_int4(0, 0, 0, 0);
         if (x < nq) {
           const int node = (x0 + x) / G, h = (x0 + x) % G;
@@ -326,7 +322,7 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
         if ((l & 3) == 0 && s != 0) atomicAdd(&qsum[x], (unsigned long long)s);
       }
 #pragma unroll
-      for (int p = 0; p < 4; p++) qf[((mt * KS + ks) * 4 + p) * 32 + l] = make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
+      for (int p = 0; p < 4; p++) qf[(ks * 4 + p) * 32 + l] = make_uint4(pl[0][p], pl[1][p], pl[2][p], pl[3][p]);
     }
   const bool q3 = __syncthreads_or(top);   // some query has a fourth digit
   if (bounds[0] < 0) {   // the parents are out of range (for the whole cluster)
@@ -347,82 +343,69 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   // ---- scores of slots [cb, cb + len) into sc, the rows' maxima into mx
   auto scores = [&](int cb, int len, bool want_max) {
     const int nt = ((len + 31) & ~31) / 8;
-    int32_t lmax[MT][2];
+    int32_t lmax[2] = {UNSEEN, UNSEEN};
+    // K in runs of one or two steps of columns, two runs on their way in turn (a run waits as one: a warp
+    // has six load counters, and more of them rolling would wait for each other)
+    int4 kb[2][KG][2];
+    auto load = [&](int4 (&b)[KG][2], const int32_t *p) {
 #pragma unroll
-    for (int m = 0; m < MT; m++) lmax[m][0] = lmax[m][1] = UNSEEN;
-    // a warp's K rows come in runs of up to four steps (4 KB), which wait as one: the next run leaves once
-    // this one is multiplied, and the SM's other fifteen warps' runs fill the time
-    int4 kb[KG][2];
-    auto load = [&](const int32_t *p) {
-#pragma unroll
-      for (int i = 0; i < KG; i++) ld_kv8(kb[i][0], kb[i][1], p + i * 32);
+      for (int i = 0; i < KG; i++) ld_kv8(b[i][0], b[i][1], p + i * 32);
     };
     auto row_of = [&](int t) { return q.kv.k + (size_t)rows[t * 8 + n8] * HD + 8 * c4; };
     const float scale = __fmul_rn(a.ascale, 0x1p-18f);   // score on the 2^32 grid -> units of 2^-14
     const int32_t *kr = q.kv.k;
     if (warp < nt) {
       kr = row_of(warp);
-      load(kr);
+      load(kb[0], kr);
+      load(kb[1], kr + KG * 32);
     }
 #pragma unroll 1
     for (int t = warp; t < nt; t += NW) {
       const int32_t *kn = row_of(min(t + NW, nt - 1));
-      int32_t acc[MT][7][4];
+      int32_t acc[7][4];
 #pragma unroll
-      for (int m = 0; m < MT; m++)
+      for (int c = 0; c < 7; c++)
 #pragma unroll
-        for (int c = 0; c < 7; c++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) acc[m][c][i] = 0;
+        for (int i = 0; i < 4; i++) acc[c][i] = 0;
 #pragma unroll
       for (int k0 = 0; k0 < KS; k0 += KG) {
+        int4(&kc)[KG][2] = kb[k0 / KG & 1];
         uint32_t k3 = 0u;
 #pragma unroll
         for (int i = 0; i < KG; i++) {
           uint32_t b0[4], b1[4];
-          digits(kb[i][0].x, kb[i][0].y, kb[i][0].z, kb[i][0].w, b0);
-          digits(kb[i][1].x, kb[i][1].y, kb[i][1].z, kb[i][1].w, b1);
+          digits(kc[i][0].x, kc[i][0].y, kc[i][0].z, kc[i][0].w, b0);
+          digits(kc[i][1].x, kc[i][1].y, kc[i][1].z, kc[i][1].w, b1);
           k3 |= b0[3] | b1[3];
 #pragma unroll
-          for (int p = 0; p < 3; p++)
+          for (int p = 0; p < 3; p++) {
+            const uint4 A = qf[((k0 + i) * 4 + p) * 32 + lane];
 #pragma unroll
-            for (int m = 0; m < MT; m++) {
-              const uint4 A = qf[((m * KS + k0 + i) * 4 + p) * 32 + lane];
-#pragma unroll
-              for (int j = 0; j < 3; j++) mma_su(acc[m][p + j], A, b0[j], b1[j]);
-            }
-        }
-        if (__any_sync(0xffffffffu, k3 != 0u) || q3) {   // fourth digits
-#pragma unroll 1
-          for (int i = 0; i < KG; i++) {
-            int4 v0 = kb[0][0], v1 = kb[0][1];
-#pragma unroll
-            for (int j = 1; j < KG; j++)
-              if (i == j) { v0 = kb[j][0]; v1 = kb[j][1]; }
-            uint32_t b0[4], b1[4];
-            digits(v0.x, v0.y, v0.z, v0.w, b0);
-            digits(v1.x, v1.y, v1.z, v1.w, b1);
-#pragma unroll
-            for (int m = 0; m < MT; m++) {
-#pragma unroll
-              for (int p = 0; p < 4; p++)
-                mma_ss(acc[m][p + 3], qf[((m * KS + k0 + i) * 4 + p) * 32 + lane], b0[3], b1[3]);
-              const uint4 A = qf[((m * KS + k0 + i) * 4 + 3) * 32 + lane];
-#pragma unroll
-              for (int j = 0; j < 3; j++) mma_su(acc[m][3 + j], A, b0[j], b1[j]);
-            }
+            for (int j = 0; j < 3; j++) mma_su(acc[p + j], A, b0[j], b1[j]);
           }
         }
-        load(k0 + KG < KS ? kr + (k0 + KG) * 32 : kn);
+        if (__any_sync(0xffffffffu, k3 != 0u) || q3) {   // fourth digits
+#pragma unroll
+          for (int i = 0; i < KG; i++) {
+            uint32_t b0[4], b1[4];
+            digits(kc[i][0].x, kc[i][0].y, kc[i][0].z, kc[i][0].w, b0);
+            digits(kc[i][1].x, kc[i][1].y, kc[i][1].z, kc[i][1].w, b1);
+#pragma unroll
+            for (int p = 0; p < 4; p++) mma_ss(acc[p + 3], qf[((k0 + i) * 4 + p) * 32 + lane], b0[3], b1[3]);
+            const uint4 A = qf[((k0 + i) * 4 + 3) * 32 + lane];
+#pragma unroll
+            for (int j = 0; j < 3; j++) mma_su(acc[3 + j], A, b0[j], b1[j]);
+          }
+        }
+        const int kx = k0 + 2 * KG;
+        load(kc, kx < KS ? kr + kx * 32 : kn + (kx - KS) * 32);
       }
       kr = kn;
       const int slot = cb + t * 8 + 2 * c4;   // this lane's two slots
       const bool all = cb + t * 8 >= clear && cb + t * 8 + 8 <= min(q.ctx, c1);
 #pragma unroll
-      for (int m = 0; m < MT; m++)
-#pragma unroll
         for (int h = 0; h < 2; h++) {
-          const int x = m * 16 + n8 + h * 8;
+          const int x = n8 + h * 8;
           const int64_t off = -BIAS * (int64_t)qsum[x];
           int32_t z[2];
           bool see[2] = {true, true};
@@ -436,11 +419,11 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
 #pragma unroll
           for (int i = 0; i < 2; i++) {
             const int e = 2 * h + i;
-            int64_t s = off + acc[m][0][e];
-            s += (int64_t)acc[m][1][e] * 256;
-            s += (int64_t)acc[m][2][e] * 65536;
-            s += (int64_t)acc[m][3][e] * 16777216;
-            s += (int64_t)(acc[m][4][e] + acc[m][5][e] * 256 + acc[m][6][e] * 65536) << 32;
+            int64_t s = off + acc[0][e];
+            s += (int64_t)acc[1][e] * 256;
+            s += (int64_t)acc[2][e] * 65536;
+            s += (int64_t)acc[3][e] * 16777216;
+            s += (int64_t)(acc[4][e] + acc[5][e] * 256 + acc[6][e] * 65536) << 32;
             // f32 of the score (one rounding: below 2^53 wherever |z| < 2^17), then z 2^14 rounded half
             // away from zero: adding a half towards zero never crosses a whole number
             float v = __fmul_rn(__ll2float_rn(s), scale);
@@ -449,124 +432,144 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
               v = 0.0f;
             }
             z[i] = see[i] ? __float2int_rz(__fadd_rz(v, copysignf(0.5f, v))) : UNSEEN;
-            lmax[m][h] = max(lmax[m][h], z[i]);
+            lmax[h] = max(lmax[h], z[i]);
           }
-          *reinterpret_cast<int2 *>(sc + x * SCS + t * 8 + 2 * c4) = make_int2(z[0], z[1]);
+          // slots 8 (t % 4) + 2 c4 .. of block t / 4: half (t % 4) / 2, lane 4 n8 + (2 (t % 2) + c4 / 2)
+          int32_t *to = sc + (t >> 2) * 512 + ((t >> 1) & 1) * 256 + h * 128;
+          *reinterpret_cast<int2 *>(to + (4 * n8 + 2 * (t & 1) + (c4 >> 1)) * 4 + 2 * (c4 & 1)) = make_int2(z[0], z[1]);
         }
     }
     if (want_max) {
 #pragma unroll
-      for (int m = 0; m < MT; m++)
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-          int32_t v = lmax[m][h];
+      for (int h = 0; h < 2; h++) {
+          int32_t v = lmax[h];
           v = max(v, __shfl_xor_sync(0xffffffffu, v, 1));
           v = max(v, __shfl_xor_sync(0xffffffffu, v, 2));
-          if (c4 == 0 && v != UNSEEN) atomicMax(&mx[m * 16 + n8 + h * 8], v);
-        }
-    }
-    __syncthreads();
-  };
-
-  // ---- exponentials in place: four neighbours' scores become their bytes' planes
-  auto exps = [&](int len) {
-    for (int x = warp; x < QV; x += NW) {
-      const int32_t m = mx[x];
-      int64_t sum = 0;
-      for (int i = lane; i < ((len + 31) & ~31) / 4; i += 32) {
-        int4 *p = reinterpret_cast<int4 *>(sc + x * SCS) + i;
-        const int4 z = *p;
-        const uint32_t e0 = exp_grid(z.x, m), e1 = exp_grid(z.y, m), e2 = exp_grid(z.z, m), e3 = exp_grid(z.w, m);
-        sum += (int64_t)e0 + e1 + (int64_t)e2 + e3;
-        *reinterpret_cast<uint4 *>(p) = bytes4(e0, e1, e2, e3);
+          if (c4 == 0 && v != UNSEEN) atomicMax(&mx[n8 + h * 8], v);
       }
-      sum = warp_sum_i64(sum);
-      if (lane == 0) ssum[x] += sum;
     }
     __syncthreads();
   };
 
-  // ---- V-sums: warp (dg, pg) takes dims dg 8 ND .. of the pass over every PG-th run of 32 slots
+  // ---- exponentials in place, a block of 16 x 32 by a warp: a lane's four quarters are its four registers
+  // of the row operand, four neighbours' bytes each, and leave as planes
+  auto exps = [&](int len) {
+    int64_t sum[2] = {0, 0};
+#pragma unroll 1
+    for (int i = warp; i < (len + 31) / 32; i += NW) {
+      const int32_t m0 = mx[n8], m1 = mx[n8 + 8];
+      int4 *p = reinterpret_cast<int4 *>(sc + i * 512) + lane;
+      uint4 r[4];
+      int64_t s0 = 0, s1 = 0;
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        const int4 z = p[u * 32];
+        const int32_t mm = u & 1 ? m1 : m0;
+        const uint32_t e0 = exp_grid(z.x, mm), e1 = exp_grid(z.y, mm), e2 = exp_grid(z.z, mm), e3 = exp_grid(z.w, mm);
+        const int64_t s = ((int64_t)e0 + e1) + ((int64_t)e2 + e3);
+        if (u & 1) s1 += s;
+        else s0 += s;
+        r[u] = bytes4(e0, e1, e2, e3);
+      }
+      uint4 *o = reinterpret_cast<uint4 *>(p);
+      o[0] = make_uint4(r[0].x, r[1].x, r[2].x, r[3].x);
+      o[32] = make_uint4(r[0].y, r[1].y, r[2].y, r[3].y);
+      o[64] = make_uint4(r[0].z, r[1].z, r[2].z, r[3].z);
+      o[96] = make_uint4(r[0].w, r[1].w, r[2].w, r[3].w);
+      sum[0] += s0;
+      sum[1] += s1;
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      int64_t s = sum[h];
+      s += __shfl_xor_sync(0xffffffffu, s, 1);
+      s += __shfl_xor_sync(0xffffffffu, s, 2);
+      if (c4 == 0 && s != 0) atomicAdd(&ssum[n8 + 8 * h], (unsigned long long)s);
+    }
+    __syncthreads();
+  };
+
+  // ---- V-sums: warp (dg, pg) takes dims 16 dg .. over every PG-th run of 32 slots
   const int dg = warp % T::DG, pg = warp / T::DG;
-  int32_t acc[MT][ND][7][4];
-  int32_t vv[2][4][ND];   // a run's V rows, on their way while the run before is multiplied
-  auto vload = [&](int st, int nst, int d0) {
-    const int32_t *vb = q.kv.v + d0 + dg * 8 * ND + ND * n8;
+  int32_t acc[ND][7][4];
+  int32_t va[2][4][ND], vb[2][4][ND];   // two runs' V rows, on their way while the run before is multiplied
+  auto vload = [&](int32_t (&v)[2][4][ND], int st, int nst) {
+    const int32_t *base = q.kv.v + dg * 8 * ND + ND * n8;
     st = min(st, nst - 1);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const uint4 r = *reinterpret_cast<const uint4 *>(rows + st * 32 + h * 16 + 4 * c4);
-      ld_kv<ND>(vv[h][0], vb + (size_t)r.x * HD);
-      ld_kv<ND>(vv[h][1], vb + (size_t)r.y * HD);
-      ld_kv<ND>(vv[h][2], vb + (size_t)r.z * HD);
-      ld_kv<ND>(vv[h][3], vb + (size_t)r.w * HD);
+      ld_kv2(v[h][0], base + (size_t)r.x * HD);
+      ld_kv2(v[h][1], base + (size_t)r.y * HD);
+      ld_kv2(v[h][2], base + (size_t)r.z * HD);
+      ld_kv2(v[h][3], base + (size_t)r.w * HD);
     }
   };
-  auto vsums = [&](int len, int d0) {   // (the first run's rows are on their way)
+  auto vfirst = [&](int len) {
+    if (len <= 0) return;
+    vload(va, pg, (len + 31) / 32);
+    vload(vb, pg + T::PG, (len + 31) / 32);
+  };
+  auto vsums = [&](int len) {   // (the first two runs' rows are on their way)
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int d = 0; d < ND; d++)
 #pragma unroll
-      for (int d = 0; d < ND; d++)
+      for (int c = 0; c < 7; c++)
 #pragma unroll
-        for (int c = 0; c < 7; c++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) acc[m][d][c][i] = 0;
+        for (int i = 0; i < 4; i++) acc[d][c][i] = 0;
     const int nst = (len + 31) / 32;
-#pragma unroll 1
-    for (int st = pg; st < nst; st += T::PG) {
+    auto step = [&](int32_t (&v)[2][4][ND], int st) {
       uint32_t b[ND][2][4], v3 = 0u;   // [dim][half][plane]
 #pragma unroll
       for (int d = 0; d < ND; d++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          digits(vv[h][0][d], vv[h][1][d], vv[h][2][d], vv[h][3][d], b[d][h]);
+          digits(v[h][0][d], v[h][1][d], v[h][2][d], v[h][3][d], b[d][h]);
           v3 |= b[d][h][3];
         }
-      vload(st + T::PG, nst, d0);
+      vload(v, st + 2 * T::PG, nst);
       const bool any3 = __any_sync(0xffffffffu, v3 != 0u);
+      const uint4 *A = reinterpret_cast<const uint4 *>(sc + st * 512) + lane;
 #pragma unroll
-      for (int m = 0; m < MT; m++) {
-        const uint32_t *e = reinterpret_cast<const uint32_t *>(sc) + (m * 16 + n8) * SCS + st * 32 + 4 * c4;
-        const uint4 r0 = *reinterpret_cast<const uint4 *>(e), r1 = *reinterpret_cast<const uint4 *>(e + 8 * SCS);
-        const uint4 r2 = *reinterpret_cast<const uint4 *>(e + 16), r3 = *reinterpret_cast<const uint4 *>(e + 8 * SCS + 16);
-        const uint4 A[4] = {make_uint4(r0.x, r1.x, r2.x, r3.x), make_uint4(r0.y, r1.y, r2.y, r3.y),
-                            make_uint4(r0.z, r1.z, r2.z, r3.z), make_uint4(r0.w, r1.w, r2.w, r3.w)};
+      for (int p = 0; p < 4; p++) {
+        const uint4 e = A[p * 32];
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+          for (int j = 0; j < 3; j++) mma_uu(acc[d][p + j], e, b[d][0][j], b[d][1][j]);
+      }
+      if (any3) {
 #pragma unroll
         for (int p = 0; p < 4; p++)
 #pragma unroll
-          for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int j = 0; j < 3; j++) mma_uu(acc[m][d][p + j], A[p], b[d][0][j], b[d][1][j]);
-        if (any3) {
-#pragma unroll
-          for (int p = 0; p < 4; p++)
-#pragma unroll
-            for (int d = 0; d < ND; d++) mma_us(acc[m][d][p + 3], A[p], b[d][0][3], b[d][1][3]);
-        }
+          for (int d = 0; d < ND; d++) mma_us(acc[d][p + 3], A[p * 32], b[d][0][3], b[d][1][3]);
       }
+    };
+#pragma unroll 1
+    for (int st = pg; st < nst; st += 2 * T::PG) {
+      step(va, st);
+      if (st + T::PG < nst) step(vb, st + T::PG);
     }
   };
   // V-sum = lo + hi 2^32: four classes below 2^31 each fit lo with room for every rank's, three fit hi
-  auto fold = [&](int m, int d, int i) {
-    const int32_t(&c)[7][4] = acc[m][d];
+  auto fold = [&](int d, int i) {
+    const int32_t(&c)[7][4] = acc[d];
     longlong2 r;
     r.x = c[0][i] + (long long)c[1][i] * 256 + (long long)c[2][i] * 65536 + (long long)c[3][i] * 16777216;
     r.y = c[4][i] + (long long)c[5][i] * 256 + (long long)c[6][i] * 65536;
     return r;
   };
-  auto each = [&](auto &&f) {   // (query vector, dim inside the pass, V-sum) of this lane's accumulators
+  auto each = [&](auto &&f) {   // (query vector, dim, V-sum) of this lane's accumulators
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int d = 0; d < ND; d++)
 #pragma unroll
-      for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) f(m * 16 + n8 + (i >> 1) * 8, dg * 8 * ND + ND * (2 * c4 + (i & 1)) + d, fold(m, d, i));
+      for (int i = 0; i < 4; i++) f(n8 + (i >> 1) * 8, dg * 8 * ND + ND * (2 * c4 + (i & 1)) + d, fold(d, i));
   };
 
   if (!MULTI) {   // (the launch gave every rank CS slots at most)
     if (c0 < c1) locate(c0, c1 - c0);
     scores(c0, c1 - c0, true);
-    if (c0 < c1) vload(pg, (c1 - c0 + 31) / 32, 0);   // across the exchange and the exponentials
+    vfirst(c1 - c0);   // across the exchange and the exponentials
   } else {
     for (int cb = c0; cb < c1; cb += CS) {
       locate(cb, min(CS, c1 - cb));
@@ -592,31 +595,23 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
       locate(cb, len);
       scores(cb, len, false);
       exps(len);
-#pragma unroll 1
-      for (int ps = 0; ps < T::PASSES; ps++) {
-        vload(pg, (len + 31) / 32, ps * T::DP);
-        vsums(len, ps * T::DP);
-        for (int r = 0; r < T::PG; r++) {   // (the slot groups add to the same sums in turn)
-          if (pg == r)
-            each([&](int x, int d, longlong2 v) {
-              longlong2 &k = keep[x * HD + ps * T::DP + d];
-              k.x += v.x;
-              k.y += v.y;
-            });
-          if (T::PG > 1) __syncthreads();
-        }
+      vfirst(len);
+      vsums(len);
+      for (int r = 0; r < T::PG; r++) {   // (the slot groups add to the same sums in turn)
+        if (pg == r)
+          each([&](int x, int d, longlong2 v) {
+            longlong2 &k = keep[x * HD + d];
+            k.x += v.x;
+            k.y += v.y;
+          });
+        if (T::PG > 1) __syncthreads();
       }
     }
   } else {
     exps(c1 - c0);
-#pragma unroll 1
-    for (int ps = 0; ps < T::PASSES; ps++) {
-      if (ps > 0 && c0 < c1) vload(pg, (c1 - c0 + 31) / 32, ps * T::DP);
-      vsums(c1 - c0, ps * T::DP);
-      if (ps + 1 < T::PASSES) each([&](int x, int d, longlong2 v) { keep[(ps * QV + x) * T::DP + d] = v; });
-    }
+    vsums(c1 - c0);
   }
-  // ---- join: dim d's sums go to rank d / DPR; the last pass straight from registers
+  // ---- join: dim d's sums go to rank d / DPR, straight from registers
   if (CL > 1) cluster.sync();   // every rank is done with its scores: their memory takes the sums
   else __syncthreads();
   const int DPR = HD / CL, lg = 31 - __clz(DPR), src = MULTI ? 1 : T::PG;   // (a power of two; sums per rank)
@@ -628,40 +623,36 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   if (MULTI) {
     for (int i = tid; i < QV * HD; i += TT) push(i / HD, i % HD, keep[i]);
   } else {
-    each([&](int x, int d, longlong2 v) { push(x, (T::PASSES - 1) * T::DP + d, v); });
-    for (int i = tid; i < (T::PASSES - 1) * QV * T::DP; i += TT) {   // (PG is 1 with passes)
-      const int ps = i / (QV * T::DP), r = i % (QV * T::DP);
-      push(r / T::DP, ps * T::DP + r % T::DP, keep[i]);
-    }
+    each(push);
   }
-  static_assert(T::PASSES == 1 || T::PG == 1, "one slot group where there are passes");
   if (CL > 1) {
     for (int i = tid; i < CL * QV; i += TT) *cluster.map_shared_rank(&s_in[rank][i % QV], i / QV) = ssum[i % QV];
     cluster.sync();   // the last cluster access
     if (tid < QV) {
-      long long s = 0;
+      unsigned long long s = 0;
       for (int r = 0; r < CL; r++) s += s_in[r][tid];
       ssum[tid] = s;
     }
   }
-  if (tid < QV) rinv[tid] = __ddiv_rn(65536.0, __ll2double_rn(ssum[tid]));
+  if (tid < QV) rinv[tid] = __ddiv_rn(65536.0, __ull2double_rn(ssum[tid]));
   __syncthreads();
+#pragma unroll 2
   for (int i = tid; i < nq << lg; i += TT) {
-    const int x = i >> lg, d = i & (DPR - 1), node = (x0 + x) / G, h = (x0 + x) % G;
+    const int x = i >> lg, d = i & (DPR - 1);
     long long lo = 0, hi = 0;
     for (int r = 0; r < CL * src; r++) {
       const longlong2 v = sums[((r * QV + x) << lg) | d];
       lo += v.x;
       hi += v.y;
     }
-    const long long S = ssum[x];
+    const long long S = (long long)ssum[x];
     acc128 N{0ull, 0ll};   // lo + hi 2^32 - BIAS sum e
     acc128_add(N, lo);
     acc128_add(N, acc128{(uint64_t)hi << 32, hi >> 32});
     acc128_add(N, acc128{(uint64_t)(-BIAS * S), __mul64hi(-BIAS, S)});
     const float o = finish(N, (uint64_t)S, rinv[x]);
-    a.out[((size_t)(q.row0 + node) * a.NH + (size_t)g * G + h) * HD + rank * DPR + d] = o;
-    if (a.ao_max) atomicMax(&omx[node - x0 / G], __float_as_uint(fabsf(o)));   // (a tile may begin inside a node's heads)
+    a.out[(size_t)out_at[x] * HD + rank * DPR + d] = o;
+    if (a.ao_max) atomicMax(&omx[node_of[x]], __float_as_uint(fabsf(o)));
   }
   if (a.ao_max) {
     __syncthreads();
@@ -769,10 +760,10 @@ namespace {
 // as much time as.
 constexpr int TREE_FIXED = 256;
 
-template <int HD, int MT, bool MULTI>
+template <int HD, bool MULTI>
 cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, int span, cudaStream_t st) {
-  using T = TreeTile<HD, MT, MULTI>;
-  auto kern = k_tree_attn<HD, MT, MULTI>;
+  using T = TreeTile<HD, MULTI>;
+  auto kern = k_tree_attn<HD, MULTI>;
   // CTAs that run at once, by cluster size (asked once per device, before any launch: a capture never
   // sees a failed launch)
   static int room[64][5];
@@ -813,25 +804,21 @@ cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, int span, cudaStre
     if (best < 0 || c < cost) { best = i; cost = c; }
   }
   if (best < 0) return cudaErrorInvalidValue;
-  return launch(kern, dim3(1 << best, a.c.NKV, (unsigned)tiles), dim3(T::TT), T::SMEM, 1 << best, st, a, 1 << best);
+  return launch(kern, dim3((unsigned)(tiles << best), a.c.NKV), dim3(T::TT), T::SMEM, 1 << best, st, a, 1 << best);
 }
 
 template <int HD>
 cudaError_t tree_attn_hd(const TreeAttnArgs &a, cudaStream_t st) {
   const int G = a.NH / a.c.NKV;
-  // two row tiles per CTA where a sequence's queries fill them; more slots than a cluster of 16 keeps
-  // scores for go in runs
+  // more slots than a cluster of 16 keeps scores for go in runs
   const int span = (a.win >= 0 && a.win < a.max_ctx ? a.win : a.max_ctx) + TREE_NODES;
-  const bool multi = span > 16 * TreeTile<HD, 1, false>::CS;
-  const bool two = !multi && (long long)a.c.rows * G > 16ll * a.c.n_seq;
-  const int QV = two ? 32 : 16;
   // tiles: every sequence's last one may be partly filled
+  constexpr int QV = TreeTile<HD, false>::QV;
   const long long most = (long long)a.c.n_seq * ((TREE_NODES * G + QV - 1) / QV);
   long long tiles = a.c.n_seq == 1 ? ((long long)a.c.rows * G + QV - 1) / QV : (long long)a.c.rows * G / QV + a.c.n_seq;
   if (tiles > most) tiles = most;
-  if (tiles > 65535) return cudaErrorInvalidValue;
-  if (multi) return tree_attn<HD, 1, true>(a, tiles, span, st);
-  return two ? tree_attn<HD, 2, false>(a, tiles, span, st) : tree_attn<HD, 1, false>(a, tiles, span, st);
+  return span > 16 * TreeTile<HD, false>::CS ? tree_attn<HD, true>(a, tiles, span, st)
+                                             : tree_attn<HD, false>(a, tiles, span, st);
 }
 
 }  // namespace
