@@ -177,6 +177,7 @@ struct TreeTile {
   static constexpr size_t SC = (size_t)QV * CS * 4;
   static constexpr size_t WORK = SC + CS * 4;
   static constexpr size_t POST = SUMS * (MULTI ? 1 : PG);       // over the scores: every source's sums of this rank's dims
+  static constexpr int BESIDE = MULTI ? 0 : (int)((SC - POST) / (QV * 4)) & ~31;   // slots that leave room for the sums
   static constexpr size_t SMEM = HEAD + (WORK > POST ? WORK : POST);
 };
 
@@ -195,7 +196,7 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   __shared__ unsigned long long anc[TREE_NODES];
   __shared__ int32_t first[QV];
   __shared__ unsigned long long seen[QV];
-  __shared__ int32_t bounds[2];                                 // the tile's first slot, its latest window start
+  __shared__ int32_t bounds[2];                                 // -1: bad parents; the tile's latest window start
   __shared__ int32_t mx[QV], mx_in[16][QV];
   __shared__ unsigned long long ssum[QV], s_in[16][QV], qsum[QV];
   __shared__ uint32_t omx[QV];
@@ -237,6 +238,36 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   if (tile < 0) return;   // (the whole cluster)
   const int x0 = tile * QV, nq = min(QV, q.n * G - x0);   // this tile's query vectors: x -> node x / G, head x % G
 
+  // ---- this rank's slots [c0, c1): from where the window of a first token begins (deeper nodes' begin later)
+  if (CL > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+  const int u0 = a.win < 0 ? 0 : max(0, q.ctx - a.win + 1), u1 = q.ctx + q.n;
+  const int span = ((u1 - u0 + CL - 1) / CL + 31) & ~31;
+  const int c0 = min(u0 + rank * span, u1), c1 = min(c0 + span, u1);
+
+  auto locate = [&](int cb, int len) {   // the rows of slots [cb, cb + len), the last one again up to a multiple of 32
+    for (int i = tid; i < ((len + 31) & ~31); i += TT)
+      rows[i] = (uint32_t)(tree_row(a.c, q.kv, a.layer, g, cb + min(i, len - 1), a.err) / HD);
+    __syncthreads();
+  };
+
+  // K in runs of one or two steps of columns, two runs on their way in turn (a run waits as one: a warp has
+  // six load counters, and more of them rolling would wait for each other)
+  int4 kb[2][KG][2];
+  auto load = [&](int4 (&b)[KG][2], const int32_t *p) {
+#pragma unroll
+    for (int i = 0; i < KG; i++) ld_kv8(b[i][0], b[i][1], p + i * 32);
+  };
+  auto row_of = [&](int t) { return q.kv.k + (size_t)rows[t * 8 + n8] * HD + 8 * c4; };
+  auto kfirst = [&](int len) {
+    if (warp < ((len + 31) & ~31) / 8) {
+      load(kb[0], row_of(warp));
+      load(kb[1], row_of(warp) + KG * 32);
+    }
+  };
+
+  if (c0 < c1) locate(c0, min(CS, c1 - c0));
+  kfirst(min(CS, c1 - c0));   // across the queries' and parents' loads
+
   // ---- warp 0: ancestors by doubling, then every query vector's window and tree slots
   bool bad = false;
   if (warp == 0) {
@@ -271,7 +302,7 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
       }
       __syncwarp();
     }
-    int f = q.ctx, lo = q.ctx, hi = 0;
+    int f = q.ctx, hi = 0;
     unsigned long long m = 0;
     if (lane < nq) {
       m = anc[(x0 + lane) / G];
@@ -282,7 +313,6 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
           const int j = __ffsll((long long)b) - 1;
           if (q.ctx + __popcll(anc[j]) - 1 < f) m &= ~(1ull << j);
         }
-      lo = min(f, q.ctx);
       hi = f;
     }
     if (lane < QV) {
@@ -291,12 +321,8 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
       node_of[lane] = (x0 + lane) / G - x0 / G;              // (a tile may begin inside a node's heads)
       out_at[lane] = (q.row0 + (x0 + lane) / G) * a.NH + g * G + (x0 + lane) % G;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    if (lane == 0) { bounds[0] = bad ? -1 : lo; bounds[1] = hi; }
+    hi = __reduce_max_sync(0xffffffffu, hi);
+    if (lane == 0) { bounds[0] = bad ? -1 : 0; bounds[1] = hi; }
   }
   // ---- the other warps: the queries' digit planes in the row operand's order, and their sums
   bool top = false;
@@ -327,38 +353,17 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   const bool q3 = __syncthreads_or(top);   // some query has a fourth digit
   if (bounds[0] < 0) {   // the parents are out of range (for the whole cluster)
     if (tid == 0) raise_err(a.err, ERR_TREE);
+    if (CL > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     return;
   }
-  if (CL > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
-  const int u0 = bounds[0], u1 = q.ctx + q.n, clear = bounds[1];
-  const int span = ((u1 - u0 + CL - 1) / CL + 31) & ~31;        // this rank's slots [c0, c1)
-  const int c0 = min(u0 + rank * span, u1), c1 = min(c0 + span, u1);
+  const int clear = bounds[1];
 
-  auto locate = [&](int cb, int len) {   // the rows of slots [cb, cb + len), the last one again up to a multiple of 32
-    for (int i = tid; i < ((len + 31) & ~31); i += TT)
-      rows[i] = (uint32_t)(tree_row(a.c, q.kv, a.layer, g, cb + min(i, len - 1), a.err) / HD);
-    __syncthreads();
-  };
-
-  // ---- scores of slots [cb, cb + len) into sc, the rows' maxima into mx
+  // ---- scores of slots [cb, cb + len) into sc, the rows' maxima into mx (the first rows are on their way)
   auto scores = [&](int cb, int len, bool want_max) {
     const int nt = ((len + 31) & ~31) / 8;
     int32_t lmax[2] = {UNSEEN, UNSEEN};
-    // K in runs of one or two steps of columns, two runs on their way in turn (a run waits as one: a warp
-    // has six load counters, and more of them rolling would wait for each other)
-    int4 kb[2][KG][2];
-    auto load = [&](int4 (&b)[KG][2], const int32_t *p) {
-#pragma unroll
-      for (int i = 0; i < KG; i++) ld_kv8(b[i][0], b[i][1], p + i * 32);
-    };
-    auto row_of = [&](int t) { return q.kv.k + (size_t)rows[t * 8 + n8] * HD + 8 * c4; };
     const float scale = __fmul_rn(a.ascale, 0x1p-18f);   // score on the 2^32 grid -> units of 2^-14
-    const int32_t *kr = q.kv.k;
-    if (warp < nt) {
-      kr = row_of(warp);
-      load(kb[0], kr);
-      load(kb[1], kr + KG * 32);
-    }
+    const int32_t *kr = warp < nt ? row_of(warp) : q.kv.k;
 #pragma unroll 1
     for (int t = warp; t < nt; t += NW) {
       const int32_t *kn = row_of(min(t + NW, nt - 1));
@@ -367,10 +372,10 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
       for (int c = 0; c < 7; c++)
 #pragma unroll
         for (int i = 0; i < 4; i++) acc[c][i] = 0;
+      uint32_t k3 = 0u;
 #pragma unroll
       for (int k0 = 0; k0 < KS; k0 += KG) {
         int4(&kc)[KG][2] = kb[k0 / KG & 1];
-        uint32_t k3 = 0u;
 #pragma unroll
         for (int i = 0; i < KG; i++) {
           uint32_t b0[4], b1[4];
@@ -384,21 +389,23 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
             for (int j = 0; j < 3; j++) mma_su(acc[p + j], A, b0[j], b1[j]);
           }
         }
-        if (__any_sync(0xffffffffu, k3 != 0u) || q3) {   // fourth digits
-#pragma unroll
-          for (int i = 0; i < KG; i++) {
-            uint32_t b0[4], b1[4];
-            digits(kc[i][0].x, kc[i][0].y, kc[i][0].z, kc[i][0].w, b0);
-            digits(kc[i][1].x, kc[i][1].y, kc[i][1].z, kc[i][1].w, b1);
-#pragma unroll
-            for (int p = 0; p < 4; p++) mma_ss(acc[p + 3], qf[((k0 + i) * 4 + p) * 32 + lane], b0[3], b1[3]);
-            const uint4 A = qf[((k0 + i) * 4 + 3) * 32 + lane];
-#pragma unroll
-            for (int j = 0; j < 3; j++) mma_su(acc[3 + j], A, b0[j], b1[j]);
-          }
-        }
         const int kx = k0 + 2 * KG;
         load(kc, kx < KS ? kr + kx * 32 : kn + (kx - KS) * 32);
+      }
+      if (__any_sync(0xffffffffu, k3 != 0u) || q3) {   // fourth digits: the rows once more (a vote per step costs 10 %)
+#pragma unroll 1
+        for (int ks = 0; ks < KS; ks++) {
+          int4 v0, v1;
+          ld_kv8(v0, v1, kr + ks * 32);
+          uint32_t b0[4], b1[4];
+          digits(v0.x, v0.y, v0.z, v0.w, b0);
+          digits(v1.x, v1.y, v1.z, v1.w, b1);
+#pragma unroll
+          for (int p = 0; p < 4; p++) mma_ss(acc[p + 3], qf[(ks * 4 + p) * 32 + lane], b0[3], b1[3]);
+          const uint4 A = qf[(ks * 4 + 3) * 32 + lane];
+#pragma unroll
+          for (int j = 0; j < 3; j++) mma_su(acc[3 + j], A, b0[j], b1[j]);
+        }
       }
       kr = kn;
       const int slot = cb + t * 8 + 2 * c4;   // this lane's two slots
@@ -494,8 +501,8 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   int32_t acc[ND][7][4];
   int32_t va[2][4][ND], vb[2][4][ND];   // two runs' V rows, on their way while the run before is multiplied
   auto vload = [&](int32_t (&v)[2][4][ND], int st, int nst) {
+    if (st >= nst) return;
     const int32_t *base = q.kv.v + dg * 8 * ND + ND * n8;
-    st = min(st, nst - 1);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const uint4 r = *reinterpret_cast<const uint4 *>(rows + st * 32 + h * 16 + 4 * c4);
@@ -567,12 +574,14 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   };
 
   if (!MULTI) {   // (the launch gave every rank CS slots at most)
-    if (c0 < c1) locate(c0, c1 - c0);
     scores(c0, c1 - c0, true);
     vfirst(c1 - c0);   // across the exchange and the exponentials
   } else {
     for (int cb = c0; cb < c1; cb += CS) {
-      locate(cb, min(CS, c1 - cb));
+      if (cb > c0) {
+        locate(cb, min(CS, c1 - cb));
+        kfirst(min(CS, c1 - cb));
+      }
       scores(cb, min(CS, c1 - cb), true);
     }
   }
@@ -593,6 +602,7 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
       const int len = min(CS, c1 - cb);
       __syncthreads();
       locate(cb, len);
+      kfirst(len);
       scores(cb, len, false);
       exps(len);
       vfirst(len);
@@ -612,10 +622,14 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
     vsums(c1 - c0);
   }
   // ---- join: dim d's sums go to rank d / DPR, straight from registers
-  if (CL > 1) cluster.sync();   // every rank is done with its scores: their memory takes the sums
+  // (their memory: behind the scores, or over them once every rank is done with its own)
+  const bool beside = !MULTI && span <= T::BESIDE;
+  if (beside) sums = reinterpret_cast<longlong2 *>(raw + T::HEAD + (size_t)T::BESIDE * QV * 4);
+  else if (CL > 1) cluster.sync();
   else __syncthreads();
   const int DPR = HD / CL, lg = 31 - __clz(DPR), src = MULTI ? 1 : T::PG;   // (a power of two; sums per rank)
   auto push = [&](int x, int d, longlong2 v) {
+    if (x >= nq) return;
     longlong2 *to = sums + ((((rank * src + (MULTI ? 0 : pg)) * QV + x) << lg) | (d & (DPR - 1)));
     if (CL > 1) to = cluster.map_shared_rank(to, d >> lg);
     *to = v;
