@@ -676,7 +676,8 @@ struct spb_session {
   int32_t *nodes_dev = nullptr, *h_nodes = nullptr;   // [3][LG_MAX]: parent (or path), row, token
   float *lp_dev = nullptr;        // [LG_MAX] logprob, lse, entropy, then [LG_MAX][LOGPROB_TOP] ids and logprobs
   // the drafted tree cached behind the context, until it is committed or the slots are written again
-  std::vector<int32_t> tree;      // parents
+  int n_tree = 0;                 // nodes (0: no tree)
+  int32_t tree[TREE_NODES];       // parents
   cudaGraphExec_t step_graph = nullptr;
   size_t buf_bytes = 0;
   // tensor parallel: int64 partial sums of the K-split matrices [NT_MAX][E], this rank's LM-head
@@ -833,7 +834,7 @@ static void release_pages(spb_session *s) {
 // follows. A copy is waited for before the other holder may write its page in place again.
 static int prepare_write(spb_session *s, int pos, int n) {
   spb_kvpool *pool = s->pool;
-  s->tree.clear();   // a drafted tree behind the context is written over
+  s->n_tree = 0;   // a drafted tree behind the context is written over
   if (!pool || n <= 0) return SPB_OK;
   if (pos < 0 || pos + n > s->pmax) return set_err(SPB_ECONTEXT_FULL, "spb: context full");
   bool changed = false, copied = false;
@@ -1293,6 +1294,8 @@ extern "C" int spb_batch_tree_step(spb_session *const *ss, int B, const int32_t 
     rows += n_nodes[b];
     max_ctx = std::max(max_ctx, s->pos);
   }
+  if (max_ctx > TREE_SPAN - TREE_NODES)
+    return set_err(SPB_EUNSUPPORTED, "spb_batch_tree_step: contexts of at most %d positions", TREE_SPAN - TREE_NODES);
   CU(cudaSetDevice(lead->m->device));
   for (int b = 0; b < B; b++) {
     rc = prepare_write(ss[b], ss[b]->pos, n_nodes[b]);
@@ -1328,7 +1331,7 @@ extern "C" int spb_batch_tree_step(spb_session *const *ss, int B, const int32_t 
     o = *out;
     if (o.logprob) o.logprob = lp;
     rc = emit_out(lead, rows, 0, nlp, 0, &o);
-    if (rc) return rc;
+    if (rc) { cudaStreamSynchronize(lead->st); return rc; }   // (copies into lp may be on their way)
   }
   rc = collect_errors(lead);
   if (rc) return rc;   // no tree is cached
@@ -1338,7 +1341,8 @@ extern "C" int spb_batch_tree_step(spb_session *const *ss, int B, const int32_t 
   }
   at = 0;
   for (int b = 0; b < B; b++) {
-    ss[b]->tree.assign(parents + at, parents + at + n_nodes[b]);
+    ss[b]->n_tree = n_nodes[b];
+    memcpy(ss[b]->tree, parents + at, (size_t)n_nodes[b] * 4);
     at += n_nodes[b];
   }
   return SPB_OK;
@@ -1346,8 +1350,8 @@ extern "C" int spb_batch_tree_step(spb_session *const *ss, int B, const int32_t 
 
 extern "C" int spb_session_tree_commit(spb_session *s, const int32_t *path, int n) {
   if (!s || n < 0 || (n > 0 && !path)) return set_err(SPB_EBADARG, "spb_session_tree_commit: bad arg");
-  if (s->tree.empty()) return set_err(SPB_EBADSTATE, "spb_session_tree_commit: no tree is cached behind the context");
-  const int nodes = (int)s->tree.size();
+  if (s->n_tree == 0) return set_err(SPB_EBADSTATE, "spb_session_tree_commit: no tree is cached behind the context");
+  const int nodes = s->n_tree;
   bool moves = false;
   for (int i = 0; i < n; i++) {
     if (path[i] < 0 || path[i] >= nodes || s->tree[path[i]] != (i ? path[i - 1] : -1))
@@ -1356,9 +1360,8 @@ extern "C" int spb_session_tree_commit(spb_session *s, const int32_t *path, int 
   }
   CU(cudaSetDevice(s->m->device));
   if (moves) {
-    const std::vector<int32_t> tree = s->tree;
     const int rc = prepare_write(s, s->pos, nodes);   // a clone may share the pages by now
-    s->tree = tree;
+    s->n_tree = nodes;   // (without room for the copies the tree stays)
     if (rc) return rc;
     s->h_trees[0] = TreeSeq{s->kv, s->pos, 0, n, s->pmax};
     memcpy(s->h_nodes, path, (size_t)n * 4);
@@ -1370,7 +1373,7 @@ extern "C" int spb_session_tree_commit(spb_session *s, const int32_t *path, int 
     a.err = s->err_dev;
     CU(launch_kv_compact(a, s->st));
   }
-  s->tree.clear();
+  s->n_tree = 0;
   s->pos += n;
   const int rc = sync_pos(s);
   if (rc) return rc;
@@ -1404,7 +1407,7 @@ extern "C" int spb_session_decode_greedy(spb_session *s, int32_t token, int n_st
 extern "C" int spb_session_rewind(spb_session *s, int n) {
   if (!s) return set_err(SPB_EBADARG, "spb_session_rewind: null session");
   if (n < 0 || n > s->pos) return set_err(SPB_EBADARG, "spb_session_rewind: n > position");
-  s->tree.clear();   // a drafted tree belongs to the position it was drafted at
+  s->n_tree = 0;   // a drafted tree belongs to the position it was drafted at
   s->pos -= n;
   CU(cudaSetDevice(s->m->device));
   int rc = sync_pos(s);

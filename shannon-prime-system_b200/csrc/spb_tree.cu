@@ -155,11 +155,18 @@ __device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
 // which are whole numbers, so no split changes a byte.
 //   scores    a warp takes 8 slots at a time: their K rows go from global memory straight into the
 //             column operand (a lane's 32 bytes are eight columns of one slot, so the digit planes
-//             are a byte transpose in registers), the queries' planes wait in shared memory
+//             are a byte transpose in registers), the queries' planes wait in shared memory;
+//             9 products, 32 cycles a slot at HD 256 (18 of them the matrix units')
 //   exps      in place over the scores, each four neighbours' bytes transposed into the planes of
-//             the row operand
+//             the row operand; 7 cycles a slot
 //   V-sums    a warp takes 16 head dims over the slots of the run, V rows again straight from global
-//             memory (eight slots x two dims per lane and step)
+//             memory (eight slots x two dims per lane and step); 12 products, 46 cycles a slot (24 the
+//             matrix units')
+// Both passes wait for memory: an SM has 64 KB of rows on their way and gets 32 (K) and 23 (V) bytes a
+// cycle. Measured and not kept (64 nodes at context 8192, 217 us): 32 query vectors per CTA (364: the sums
+// spill, V comes in pieces of 32 bytes), 8 warps of twice the dims (241), V through shared memory for the
+// whole CTA (260: a barrier per step) or in a ring per warp (229: 80 KB that the L1 misses while K comes
+// in), a row's pieces fetched by neighbouring lanes and shuffled (214, small trees 2 to 4 % slower).
 // MULTI (more slots per rank than scores are kept for): the maxima first, then scores again in runs of
 // CS slots, each run's V-sums added up in shared memory.
 template <int HD, bool MULTI>
@@ -430,7 +437,7 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
             s += (int64_t)acc[1][e] * 256;
             s += (int64_t)acc[2][e] * 65536;
             s += (int64_t)acc[3][e] * 16777216;
-            s += (int64_t)(acc[4][e] + acc[5][e] * 256 + acc[6][e] * 65536) << 32;
+            s += (int64_t)((uint64_t)((uint32_t)acc[4][e] + (uint32_t)acc[5][e] * 256u + (uint32_t)acc[6][e] * 65536u) << 32);
             // f32 of the score (one rounding: below 2^53 wherever |z| < 2^17), then z 2^14 rounded half
             // away from zero: adding a half towards zero never crosses a whole number
             float v = __fmul_rn(__ll2float_rn(s), scale);
@@ -770,8 +777,10 @@ cudaError_t launch(void (*kern)(K...), dim3 grid, dim3 block, size_t smem, int c
 
 namespace {
 
-// Slots that a CTA's fixed work (finding its tile, the queries, three cluster barriers, the join) costs
-// as much time as.
+// A CTA's fixed work (finding its tile, the queries, two cluster barriers, the join: 16000 to 20000 cycles) in
+// slots of 80 cycles. 12B shape, 4 nodes: context 100 16.8 / 13.4 / 13.2 us with clusters of 1 / 4 / 8, context
+// 2048 36 / 25 / 45 with 4 / 8 / 16 (8 clusters of 16 take two waves); 64 nodes at context 8192 216 / 300 with
+// 4 / 8 (two waves and five).
 constexpr int TREE_FIXED = 256;
 
 template <int HD, bool MULTI>
@@ -817,7 +826,7 @@ cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, int span, cudaStre
     const long long c = waves * (per + TREE_FIXED);
     if (best < 0 || c < cost) { best = i; cost = c; }
   }
-  if (best < 0) return cudaErrorInvalidValue;
+  if (best < 0) return cudaErrorNotSupported;
   return launch(kern, dim3((unsigned)(tiles << best), a.c.NKV), dim3(T::TT), T::SMEM, 1 << best, st, a, 1 << best);
 }
 
@@ -831,8 +840,11 @@ cudaError_t tree_attn_hd(const TreeAttnArgs &a, cudaStream_t st) {
   const long long most = (long long)a.c.n_seq * ((TREE_NODES * G + QV - 1) / QV);
   long long tiles = a.c.n_seq == 1 ? ((long long)a.c.rows * G + QV - 1) / QV : (long long)a.c.rows * G / QV + a.c.n_seq;
   if (tiles > most) tiles = most;
-  return span > 16 * TreeTile<HD, false>::CS ? tree_attn<HD, true>(a, tiles, span, st)
-                                             : tree_attn<HD, false>(a, tiles, span, st);
+  if (span <= 16 * TreeTile<HD, false>::CS) {
+    const cudaError_t e = tree_attn<HD, false>(a, tiles, span, st);
+    if (e != cudaErrorNotSupported) return e;   // (no room for a cluster that large)
+  }
+  return tree_attn<HD, true>(a, tiles, span, st);
 }
 
 }  // namespace
