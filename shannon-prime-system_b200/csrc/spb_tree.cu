@@ -211,28 +211,36 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   __shared__ int32_t out_at[QV], node_of[QV];
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n8 = lane >> 2, c4 = lane & 3;
-  const int rank = CL > 1 ? (int)cluster.block_rank() : 0, g = blockIdx.y;
+  const int rank = CL > 1 ? (int)cluster.block_rank() : 0, g = blockIdx.x / CL % a.c.NKV;   // heads of a tile side by side
   const int G = a.NH / a.c.NKV;
   pdl_trigger();
   if (tid < QV) { mx[tid] = UNSEEN; ssum[tid] = qsum[tid] = 0ull; omx[tid] = 0u; }
   pdl_wait();
 
-  // ---- which sequence: tiles are counted over the sequences in order (every warp for itself)
+  // ---- which sequence: tiles are counted over the sequences (every warp for itself), up to 32 of them the
+  // longest contexts first: their CTAs run longest, and the short ones fill the gaps (8 sessions of 8 nodes,
+  // contexts of 128 to 8192: 196 -> 150 us)
   TreeSeq q;
   int tile = -1;
+  const int at = blockIdx.x / CL / a.c.NKV;
   for (int s0 = 0, before = 0; s0 < a.c.n_seq; s0 += 32) {
-    int n = 0;
+    int n = 0, ctx = -1;
     if (s0 + lane < a.c.n_seq) {
-      if (tree_seq(a.c, s0 + lane, a.max_ctx, q)) n = (q.n * G + QV - 1) / QV;
-      else if (warp == 0) raise_err(a.err, ERR_TREE);
+      if (tree_seq(a.c, s0 + lane, a.max_ctx, q)) {
+        n = (q.n * G + QV - 1) / QV;
+        ctx = q.ctx;
+      } else if (warp == 0) {
+        raise_err(a.err, ERR_TREE);
+      }
     }
-    int incl = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += v;
+    int excl = 0, total = 0;   // tiles of this lane's predecessors, of all 32
+    const bool sorted = a.c.n_seq <= 32;
+    for (int o = 0; o < min(32, a.c.n_seq - s0); o++) {
+      const int c = __shfl_sync(0xffffffffu, ctx, o), m = __shfl_sync(0xffffffffu, n, o);
+      total += m;
+      if (sorted ? c > ctx || (c == ctx && o < lane) : o < lane) excl += m;
     }
-    const int z = (int)(blockIdx.x / CL) - before - (incl - n);
+    const int z = at - before - excl;
     const uint32_t hit = __ballot_sync(0xffffffffu, z >= 0 && z < n);
     if (hit) {
       const int l = __ffs(hit) - 1;
@@ -240,15 +248,19 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
       tree_seq(a.c, s0 + l, a.max_ctx, q);
       break;
     }
-    before += __shfl_sync(0xffffffffu, incl, 31);
+    before += total;
   }
   if (tile < 0) return;   // (the whole cluster)
   const int x0 = tile * QV, nq = min(QV, q.n * G - x0);   // this tile's query vectors: x -> node x / G, head x % G
 
   // ---- this rank's slots [c0, c1): from where the window of a first token begins (deeper nodes' begin later)
-  if (CL > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int u0 = a.win < 0 ? 0 : max(0, q.ctx - a.win + 1), u1 = q.ctx + q.n;
   const int span = ((u1 - u0 + CL - 1) / CL + 31) & ~31;
+  if (!MULTI && span > CS) {   // (the launch gave every rank CS slots at most: not reached)
+    if (tid == 0) raise_err(a.err, ERR_TREE);
+    return;
+  }
+  if (CL > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int c0 = min(u0 + rank * span, u1), c1 = min(c0 + span, u1);
 
   auto locate = [&](int cb, int len) {   // the rows of slots [cb, cb + len), the last one again up to a multiple of 32
@@ -784,7 +796,7 @@ namespace {
 constexpr int TREE_FIXED = 256;
 
 template <int HD, bool MULTI>
-cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, int span, cudaStream_t st) {
+cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, long long likely, int span, cudaStream_t st) {
   using T = TreeTile<HD, MULTI>;
   auto kern = k_tree_attn<HD, MULTI>;
   // CTAs that run at once, by cluster size (asked once per device, before any launch: a capture never
@@ -822,12 +834,13 @@ cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, int span, cudaStre
   for (int i = 0; i < 5; i++) {
     const long long per = ((span + (1 << i) - 1) / (1 << i) + 31) & ~31;
     if (room[dev][i] <= 0 || (!MULTI && per > T::CS)) continue;
-    const long long waves = ((tiles * a.c.NKV << i) + room[dev][i] - 1) / room[dev][i];
+    const long long waves = ((likely * a.c.NKV << i) + room[dev][i] - 1) / room[dev][i];
     const long long c = waves * (per + TREE_FIXED);
     if (best < 0 || c < cost) { best = i; cost = c; }
   }
   if (best < 0) return cudaErrorNotSupported;
-  return launch(kern, dim3((unsigned)(tiles << best), a.c.NKV), dim3(T::TT), T::SMEM, 1 << best, st, a, 1 << best);
+  if (tiles * a.c.NKV << best > 0x7fffffffll) return cudaErrorInvalidValue;
+  return launch(kern, dim3((unsigned)(tiles * a.c.NKV << best)), dim3(T::TT), T::SMEM, 1 << best, st, a, 1 << best);
 }
 
 template <int HD>
@@ -840,11 +853,13 @@ cudaError_t tree_attn_hd(const TreeAttnArgs &a, cudaStream_t st) {
   const long long most = (long long)a.c.n_seq * ((TREE_NODES * G + QV - 1) / QV);
   long long tiles = a.c.n_seq == 1 ? ((long long)a.c.rows * G + QV - 1) / QV : (long long)a.c.rows * G / QV + a.c.n_seq;
   if (tiles > most) tiles = most;
+  // the tiles there are if the sequences are alike (the grid's others leave at once)
+  const long long likely = a.c.n_seq * (((long long)a.c.rows * G + (long long)QV * a.c.n_seq - 1) / ((long long)QV * a.c.n_seq));
   if (span <= 16 * TreeTile<HD, false>::CS) {
-    const cudaError_t e = tree_attn<HD, false>(a, tiles, span, st);
+    const cudaError_t e = tree_attn<HD, false>(a, tiles, likely, span, st);
     if (e != cudaErrorNotSupported) return e;   // (no room for a cluster that large)
   }
-  return tree_attn<HD, true>(a, tiles, span, st);
+  return tree_attn<HD, true>(a, tiles, likely, span, st);
 }
 
 }  // namespace
