@@ -183,7 +183,8 @@ struct TreeTile {
   static constexpr size_t HEAD = QF + (MULTI ? SUMS : 0);       // (MULTI: the running V-sums)
   static constexpr size_t SC = (size_t)QV * CS * 4;
   static constexpr size_t WORK = SC + CS * 4;
-  static constexpr size_t POST = SUMS * (MULTI ? 1 : PG);       // over the scores: every source's sums of this rank's dims
+  // over the scores: every source's sums of this rank's dims (HD / CL of them, or up to one more: CL <= 16)
+  static constexpr size_t POST = (SUMS + (size_t)16 * QV * 16) * (MULTI ? 1 : PG);
   static constexpr int BESIDE = MULTI ? 0 : (int)((SC - POST) / (QV * 4)) & ~31;   // slots that leave room for the sums
   static constexpr size_t SMEM = HEAD + (WORK > POST ? WORK : POST);
 };
@@ -646,11 +647,15 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   if (beside) sums = reinterpret_cast<longlong2 *>(raw + T::HEAD + (size_t)T::BESIDE * QV * 4);
   else if (CL > 1) cluster.sync();
   else __syncthreads();
-  const int DPR = HD / CL, lg = 31 - __clz(DPR), src = MULTI ? 1 : T::PG;   // (a power of two; sums per rank)
+  // (x / DPR as a product: x < 16 HD = 2^12 at most, and x times the reciprocal's excess stays below 2^22)
+  const int DPR = (HD + CL - 1) / CL, src = MULTI ? 1 : T::PG;   // a rank's dims; sums per rank
+  const uint32_t inv = ((1u << 22) + DPR - 1) / DPR;
+  auto by_dpr = [&](int x) { return (int)((uint32_t)x * inv >> 22); };
   auto push = [&](int x, int d, longlong2 v) {
     if (x >= nq) return;
-    longlong2 *to = sums + ((((rank * src + (MULTI ? 0 : pg)) * QV + x) << lg) | (d & (DPR - 1)));
-    if (CL > 1) to = cluster.map_shared_rank(to, d >> lg);
+    const int o = by_dpr(d);
+    longlong2 *to = sums + ((rank * src + (MULTI ? 0 : pg)) * QV + x) * DPR + (d - o * DPR);
+    if (CL > 1) to = cluster.map_shared_rank(to, o);
     *to = v;
   };
   if (MULTI) {
@@ -670,11 +675,12 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
   if (tid < QV) rinv[tid] = __ddiv_rn(65536.0, __ull2double_rn(ssum[tid]));
   __syncthreads();
 #pragma unroll 2
-  for (int i = tid; i < nq << lg; i += TT) {
-    const int x = i >> lg, d = i & (DPR - 1);
+  for (int i = tid; i < nq * DPR; i += TT) {
+    const int x = by_dpr(i), d = i - x * DPR;
+    if (rank * DPR + d >= HD) continue;   // (the last ranks' dims where HD / CL is no whole number)
     long long lo = 0, hi = 0;
     for (int r = 0; r < CL * src; r++) {
-      const longlong2 v = sums[((r * QV + x) << lg) | d];
+      const longlong2 v = sums[(r * QV + x) * DPR + d];
       lo += v.x;
       hi += v.y;
     }
@@ -801,46 +807,46 @@ cudaError_t tree_attn(const TreeAttnArgs &a, long long tiles, long long likely, 
   auto kern = k_tree_attn<HD, MULTI>;
   // CTAs that run at once, by cluster size (asked once per device, before any launch: a capture never
   // sees a failed launch)
-  static int room[64][5];
+  static int room[64][17];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   dev &= 63;
-  if (room[dev][0] == 0) {
+  if (room[dev][1] == 0) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::SMEM);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
-    for (int i = 4; i >= 0; i--) {
+    for (int i = 16; i >= 1; i--) {
       cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3(1 << i);
+      cfg.gridDim = dim3(i);
       cfg.blockDim = dim3(T::TT);
       cfg.dynamicSmemBytes = T::SMEM;
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
-      attr[0].val.clusterDim.x = 1 << i;
+      attr[0].val.clusterDim.x = i;
       attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
       cfg.attrs = attr;
       cfg.numAttrs = 1;
       int n = 0;
       if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
-      room[dev][i] = n << i;
+      room[dev][i] = n * i;
     }
     (void)cudaGetLastError();
-    if (room[dev][0] <= 0) return cudaErrorLaunchOutOfResources;
+    if (room[dev][1] <= 0) return cudaErrorLaunchOutOfResources;
   }
   // the cluster size whose waves of CTAs take the least slots one after the other
-  int best = -1;
+  int best = 0;
   long long cost = 0;
-  for (int i = 0; i < 5; i++) {
-    const long long per = ((span + (1 << i) - 1) / (1 << i) + 31) & ~31;
+  for (int i = 1; i <= 16; i++) {
+    const long long per = ((span + i - 1) / i + 31) & ~31;
     if (room[dev][i] <= 0 || (!MULTI && per > T::CS)) continue;
-    const long long waves = ((likely * a.c.NKV << i) + room[dev][i] - 1) / room[dev][i];
+    const long long waves = (likely * a.c.NKV * i + room[dev][i] - 1) / room[dev][i];
     const long long c = waves * (per + TREE_FIXED);
-    if (best < 0 || c < cost) { best = i; cost = c; }
+    if (best == 0 || c < cost) { best = i; cost = c; }
   }
-  if (best < 0) return cudaErrorNotSupported;
-  if (tiles * a.c.NKV << best > 0x7fffffffll) return cudaErrorInvalidValue;
-  return launch(kern, dim3((unsigned)(tiles * a.c.NKV << best)), dim3(T::TT), T::SMEM, 1 << best, st, a, 1 << best);
+  if (best == 0) return cudaErrorNotSupported;
+  if (tiles * a.c.NKV * best > 0x7fffffffll) return cudaErrorInvalidValue;
+  return launch(kern, dim3((unsigned)(tiles * a.c.NKV * best)), dim3(T::TT), T::SMEM, best, st, a, best);
 }
 
 template <int HD>
