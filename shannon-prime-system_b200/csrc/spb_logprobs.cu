@@ -267,6 +267,7 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
     if (tid < n) {
       const uint32_t k = list[tid];
       int above = 0;
+#pragma unroll 8
       for (int i = 0; i < n; i++) above += list[i] > k || (list[i] == k && i < tid);
       if (above == a.top - 1) bound_sh = k;
     }
@@ -305,6 +306,7 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
       for (int c = tid; c < nc; c += LT) {
         const unsigned long long k = cand[c];
         int above = 0;
+#pragma unroll 8
         for (int i = 0; i < nc; i++) above += cand[i] > k;
         if (above < a.top) best[above] = k;
       }
@@ -376,15 +378,33 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
   }
   // ---- rank 0: the alternatives of all ranks
   if (rank == 0 && a.top > 0) {
-    if (C > 1)
-      for (int i = tid; i < C * a.top; i += LT) {
-        const unsigned long long k = in_best[i / a.top][i % a.top];
-        if (k == 0ull) continue;
-        int above = 0;
-        for (int j = 0; j < C; j++)
-          for (int l = 0; l < a.top; l++) above += in_best[j][l] > k;
-        if (above < a.top) best[above] = k;   // (this rank's own have all been handed over)
+    if (C > 1) {   // lists in descending order, joined two by two, a pair by a warp
+      unsigned long long *to = cand;
+      for (int n = C; n > 1; n = (n + 1) / 2) {
+        if (2 * warp < n) {
+          unsigned long long k = 0ull, o = 0ull;
+          const int l = 2 * warp, rev = 31 - lane;
+          if (n == C) {
+            if (lane < a.top) k = in_best[l][lane];
+            if (l + 1 < n && rev < a.top) o = in_best[l + 1][rev];
+          } else {
+            const unsigned long long *from = cand + (to == cand ? 256 : 0);
+            k = from[l * 32 + lane];
+            if (l + 1 < n) o = from[(l + 1) * 32 + rev];
+          }
+          k = max(k, o);   // the larger half of the two, as a bitonic sequence
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) {
+            const unsigned long long p = __shfl_xor_sync(0xffffffffu, k, d);
+            k = (lane & d) ? min(k, p) : max(k, p);
+          }
+          if (n > 2) to[warp * 32 + lane] = k;
+          else if (lane < a.top) best[lane] = k;
+        }
+        to = to == cand ? cand + 256 : cand;
+        __syncthreads();
       }
+    }
     __syncthreads();
     if (tid < a.top) {
       const unsigned long long k = best[tid];
@@ -407,7 +427,9 @@ cudaError_t launch_logprobs(const LogprobArgs &a, cudaStream_t st) {
   // CTAs per SM (64 rows x 262144, 20 alternatives: 45 us with at most one per SM, 29 with two, 43 and 61
   // with two and four waves); many rows: a CTA each, three per SM
   int C = P;
-  while (C > 1 && (long long)a.rows * C > 2 * 148) C = (C + 1) / 2;
+  if ((long long)a.rows * C > 2 * 148) C = a.rows < 2 * 148 ? 2 * 148 / a.rows : 1;
+  const int each = (P + C - 1) / C;   // parts of a CTA, spread evenly
+  C = (P + each - 1) / each;
   static bool set[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
