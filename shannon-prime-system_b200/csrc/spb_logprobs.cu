@@ -182,7 +182,7 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
   __shared__ unsigned long long in_best[16][LOGPROB_TOP];            // every rank's best, on rank 0
   __shared__ int count, n_cand, n_win;
   __shared__ uint16_t winner[LT];
-  __shared__ float lse_sh;
+  __shared__ float m_sh, ls_sh;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = C > 1 ? (int)cluster.block_rank() : 0, row = blockIdx.x / C;
@@ -341,23 +341,22 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
     float m = -INFINITY, s = 0.0f, t = 0.0f;
     if (lane < P) { m = pm[lane]; s = ps[lane]; t = pt[lane]; }
     join_lanes<32>(m, s, t);
-    float lse = -INFINITY, ent = 0.0f;
-    if (!(s == s) || m == INFINITY) {
-      lse = ent = NAN;
-    } else if (s > 0.0f) {
-      lse = __fadd_rn(m, logf(s));
-      ent = __fsub_rn(logf(s), __fmul_rn(0.693147182f, __fdiv_rn(t, s)));
-    }
+    // (a row without entries above -inf: s 0)
+    const bool none = !(s == s) || m == INFINITY;
+    const float ls = none ? NAN : logf(s);
     if (lane == 0) {
-      lse_sh = lse;
+      m_sh = m;
+      ls_sh = ls;
       if (rank == 0) {
-        if (a.lse) a.lse[row] = lse;
-        if (a.entropy) a.entropy[row] = ent;
+        if (a.lse) a.lse[row] = none ? NAN : s > 0.0f ? __fadd_rn(m, ls) : -INFINITY;
+        if (a.entropy) a.entropy[row] = none ? NAN : s > 0.0f ? __fsub_rn(ls, __fmul_rn(0.693147182f, __fdiv_rn(t, s))) : 0.0f;
       }
     }
   }
   __syncthreads();
-  const float lse = lse_sh;
+  // x - lse as (x - m) - log(s): likely tokens keep the digits that lse has lost to m
+  const float m0 = m_sh, ls = ls_sh;
+  auto logprob = [&](float x) { return ls != ls ? NAN : x == -INFINITY ? -INFINITY : __fsub_rn(__fsub_rn(x, m0), ls); };
   // ---- this row's tokens (row 0's cluster also reports the rows that are out of range)
   for (int i = t0; i < a.n_tok; i += C * LT) {
     const int tr = i == t0 ? row0 : a.tok_row ? a.tok_row[i] : i;
@@ -368,12 +367,8 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
     if (tr != row) continue;
     const int tok = i == t0 ? tok0 : a.tok[i];
     float v = NAN;
-    if (tok >= 0 && tok < a.vocab) {
-      const float xv = i == t0 ? x0 : x[tok];
-      v = lse != lse ? NAN : xv == -INFINITY ? -INFINITY : __fsub_rn(xv, lse);
-    } else if (tok != -1) {
-      raise_err(a.err, ERR_TOKEN);
-    }
+    if (tok >= 0 && tok < a.vocab) v = logprob(i == t0 ? x0 : x[tok]);
+    else if (tok != -1) raise_err(a.err, ERR_TOKEN);
     a.logprob[i] = v;
   }
   // ---- rank 0: the alternatives of all ranks
@@ -408,9 +403,8 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
     __syncthreads();
     if (tid < a.top) {
       const unsigned long long k = best[tid];
-      const bool none = k == 0ull || lse != lse;
-      a.ids[(size_t)row * a.top + tid] = none ? -1 : (int)~(uint32_t)k;
-      a.best[(size_t)row * a.top + tid] = lse != lse ? NAN : none ? -INFINITY : __fsub_rn(key_value(k), lse);
+      a.ids[(size_t)row * a.top + tid] = k == 0ull || ls != ls ? -1 : (int)~(uint32_t)k;
+      a.best[(size_t)row * a.top + tid] = logprob(k == 0ull ? -INFINITY : key_value(k));
     }
   }
 }
