@@ -262,8 +262,10 @@ typedef struct {
  * [n_seq + 1], parent, q, out and the view's pointers are memory of the current device; nothing is
  * allocated after the first call on a device, calls on different streams are independent. A sequence
  * whose arrays are out of range raises a bit (spb_take_device_errors) and leaves its rows as they
- * were, as are rows of no sequence; a page outside the pool raises the bit and reads as page 0. The
- * bytes are those of decoding each path (sp_session.c:327-347 on the exact islands). */
+ * were, as are rows of no sequence; a page outside the pool raises the bit and reads as page 0. out
+ * overlaps no other argument. Before a call is captured, one of the same head_dim and max_ctx has run on
+ * the device (it allocates the error word and asks for the kernel's room). The bytes are those of decoding
+ * each path (sp_session.c:327-347 on the exact islands). */
 int spb_tree_attn(const spb_kv_view *kv, int layer, int n_seq, const int32_t *ctx, const int32_t *row0,
                   const int32_t *parent, int rows, int max_ctx, const int32_t *q, int n_head, int window,
                   float *out, void *stream);

@@ -1776,8 +1776,9 @@ extern "C" int spb_rope_cordic_dev(const float *v, int d, int rows, const int32_
 }
 
 // ---- verifying drafted trees over caches in the caller's memory
-// a device buffer of the current device (a host pointer would fault the GPU)
+// a buffer of 4-byte elements of the current device (a host pointer or an odd address would fault the GPU)
 static bool on_device(const void *p) {
+  if ((uintptr_t)p & 3) return false;
   cudaPointerAttributes at{};
   int dev = 0;
   if (cudaPointerGetAttributes(&at, p) != cudaSuccess || cudaGetDevice(&dev) != cudaSuccess) {
@@ -1826,7 +1827,7 @@ extern "C" int spb_tree_attn(const spb_kv_view *kv, int layer, int n_seq, const 
   if (!ctx || !row0 || !parent || !q || !out) return set_err(SPB_EBADARG, "spb_tree_attn: null arg");
   if ((uintptr_t)q & 15) return set_err(SPB_EBADARG, "spb_tree_attn: q must be 16-byte aligned");
   if (!view_on_device(kv) || !on_device(ctx) || !on_device(row0) || !on_device(parent) || !on_device(q) || !on_device(out))
-    return set_err(SPB_EBADARG, "spb_tree_attn: an argument is not memory of the current device");
+    return set_err(SPB_EBADARG, "spb_tree_attn: an argument is not memory of the current device, or not 4-byte aligned");
   uint8_t *wb;
   TreeAttnArgs a{};
   rc = work_get(256, &wb, &a.err);
@@ -1848,7 +1849,7 @@ extern "C" int spb_kv_compact(const spb_kv_view *kv, int n_seq, const int32_t *c
   if (n_path == 0) return SPB_OK;
   if (!ctx || !path0 || !path) return set_err(SPB_EBADARG, "spb_kv_compact: null arg");
   if (!view_on_device(kv) || !on_device(ctx) || !on_device(path0) || !on_device(path))
-    return set_err(SPB_EBADARG, "spb_kv_compact: an argument is not memory of the current device");
+    return set_err(SPB_EBADARG, "spb_kv_compact: an argument is not memory of the current device, or not 4-byte aligned");
   uint8_t *wb;
   KvCompactArgs a{};
   rc = work_get(256, &wb, &a.err);
@@ -1874,7 +1875,8 @@ extern "C" int spb_logprobs(const float *logits, int rows, int vocab, int64_t ld
   const void *ps[] = {logits, n_tok ? tok_row : nullptr, n_tok ? tok : nullptr, n_tok ? logprob : nullptr,
                       lse, entropy, top ? top_id : nullptr, top ? top_logprob : nullptr};
   for (const void *p : ps)
-    if (p && !on_device(p)) return set_err(SPB_EBADARG, "spb_logprobs: an argument is not memory of the current device");
+    if (p && !on_device(p))
+      return set_err(SPB_EBADARG, "spb_logprobs: an argument is not memory of the current device, or not 4-byte aligned");
   uint8_t *wb;
   LogprobArgs a{};
   const int rc = work_get(256, &wb, &a.err);

@@ -509,6 +509,30 @@ def test_logprobs_optional_outputs(cuda_ok):
     assert (got[2] == 7.0).all() and np.isfinite(got[1]).all()
 
 
+def test_odd_addresses_are_refused(cuda_ok):
+    """Device pointers off a 4-byte boundary come back as an error (the host refuses them: nothing runs)."""
+    c = Case(9, 1, 1, 64, 16, [20], [[-1, 0]]).upload()
+    d, v = {n: t.data_ptr() for n, t in c.d.items()}, c.view
+    out = torch.zeros(2, 64, device="cuda").data_ptr()
+    args = [d["ctx"], d["row0"], d["parent"], out]
+    for i in range(4):
+        a = [p + 2 * (i == j) for j, p in enumerate(args)]
+        with pytest.raises(spb200.SpbError):
+            spb200.tree_attn(v, 0, 1, a[0], a[1], a[2], 2, 20, d["q"], 1, -1, a[3])
+        if i < 3:
+            with pytest.raises(spb200.SpbError):
+                spb200.kv_compact(v, 1, a[0], a[1], a[2], 2)
+    v.ptab += 1
+    with pytest.raises(spb200.SpbError):
+        spb200.kv_compact(v, 1, d["ctx"], d["row0"], d["parent"], 2)
+    x, i32 = torch.zeros(4, 64, device="cuda").data_ptr(), torch.zeros(64, dtype=torch.int32, device="cuda").data_ptr()
+    args = [x, i32, i32, x, x, x, i32, x]
+    for i in range(8):
+        a = [p + (i == j) for j, p in enumerate(args)]
+        with pytest.raises(spb200.SpbError):
+            spb200.logprobs(a[0], 2, 64, 64, a[1], a[2], 2, a[3], a[4], a[5], 3, a[6], a[7])
+
+
 # ------------------------------------------------------------------------------ the whole step
 @pytest.fixture(scope="module", params=["micro_gemma", "micro_qwen"])
 def env(request):
