@@ -192,15 +192,6 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
   if (tid < LOGPROB_TOP) best[tid] = 0ull;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const float *x = a.x + (size_t)row * a.ld;
-  // this thread's first token of the call, if it is one of this row's, is on its way from the start
-  const int t0 = rank * LT + tid;
-  int tok0 = -1, row0 = -1;
-  float x0 = 0.0f;
-  if (t0 < a.n_tok) {
-    row0 = a.tok_row ? a.tok_row[t0] : t0;
-    tok0 = a.tok[t0];
-    if (row0 == row && tok0 >= 0 && tok0 < a.vocab) x0 = x[tok0];
-  }
   // ---- the rank's parts: part p of every C
   const int sh = (int)(((uintptr_t)x >> 2) & 3);
   float largest = -INFINITY;   // this thread's
@@ -357,17 +348,19 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
   // x - lse as (x - m) - log(s): likely tokens keep the digits that lse has lost to m
   const float m0 = m_sh, ls = ls_sh;
   auto logprob = [&](float x) { return ls != ls ? NAN : x == -INFINITY ? -INFINITY : __fsub_rn(__fsub_rn(x, m0), ls); };
-  // ---- this row's tokens (row 0's cluster also reports the rows that are out of range)
-  for (int i = t0; i < a.n_tok; i += C * LT) {
-    const int tr = i == t0 ? row0 : a.tok_row ? a.tok_row[i] : i;
+  // ---- this row's tokens: without tok_row token `row`, else every row's CTAs look through the list (row 0's
+  // cluster also reports the rows that are out of range)
+  const int t1 = a.tok_row ? a.n_tok : min(a.n_tok, row + 1);
+  for (int i = (a.tok_row ? rank * LT : rank == 0 ? row : a.n_tok) + tid; i < t1; i += C * LT) {
+    const int tr = a.tok_row ? a.tok_row[i] : row;
     if (tr < 0 || tr >= a.rows) {
       if (row == 0) { raise_err(a.err, ERR_TOKEN); a.logprob[i] = NAN; }
       continue;
     }
     if (tr != row) continue;
-    const int tok = i == t0 ? tok0 : a.tok[i];
+    const int tok = a.tok[i];
     float v = NAN;
-    if (tok >= 0 && tok < a.vocab) v = logprob(i == t0 ? x0 : x[tok]);
+    if (tok >= 0 && tok < a.vocab) v = logprob(x[tok]);
     else if (tok != -1) raise_err(a.err, ERR_TOKEN);
     a.logprob[i] = v;
   }

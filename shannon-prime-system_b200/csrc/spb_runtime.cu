@@ -1866,8 +1866,8 @@ extern "C" int spb_logprobs(const float *logits, int rows, int vocab, int64_t ld
   if (rows < 0 || vocab <= 0 || ld < vocab || n_tok < 0)
     return set_err(SPB_EBADARG, "spb_logprobs: bad arg (rows, n_tok >= 0, vocab > 0, ld >= vocab)");
   if (top < 0 || top > LOGPROB_TOP) return set_err(SPB_EBADARG, "spb_logprobs: top in [0, %d]", LOGPROB_TOP);
-  if (vocab > LOGPROB_VOCAB || rows > (1 << 26))
-    return set_err(SPB_EUNSUPPORTED, "spb_logprobs: %d entries per row and 2^26 rows at most", LOGPROB_VOCAB);
+  if (vocab > LOGPROB_VOCAB || rows > (1 << 26) || n_tok > (1 << 26))
+    return set_err(SPB_EUNSUPPORTED, "spb_logprobs: %d entries per row, 2^26 rows and 2^26 tokens at most", LOGPROB_VOCAB);
   if (rows == 0 && n_tok == 0) return SPB_OK;
   if (rows == 0 || !logits || (n_tok > 0 && (!tok || !logprob)) || (top > 0 && (!top_id || !top_logprob)))
     return set_err(SPB_EBADARG, "spb_logprobs: null arg, or tokens without rows");

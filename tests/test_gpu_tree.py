@@ -509,6 +509,142 @@ def test_logprobs_optional_outputs(cuda_ok):
     assert (got[2] == 7.0).all() and np.isfinite(got[1]).all()
 
 
+@pytest.mark.parametrize("rows,n_tok", [(700, 700), (700, 3), (9, 9), (1, 1), (2, 0)])
+def test_logprobs_token_of_its_row(cuda_ok, rows, n_tok):
+    """Without tok_row, token t is row t's; fewer tokens than rows leave the rest alone."""
+    V = 997
+    r = np.random.default_rng(5)
+    x = (r.standard_normal((rows, V)) * 2).astype(np.float32)
+    tok = r.integers(0, V, max(n_tok, 1)).astype(np.int32)
+    if n_tok > 2:
+        tok[1], tok[2] = -1, V
+    d, t, lp = dev(x), dev(tok), torch.full((max(rows, 1),), 7.0, device="cuda")
+    errs()
+    spb200.logprobs(d.data_ptr(), rows, V, V, None, t.data_ptr(), n_tok, lp.data_ptr(), None, None, 0, None, None)
+    got, want = lp.cpu().numpy(), lp_ref(x[:n_tok], range(n_tok), tok[:n_tok], 0)[0] if n_tok else np.zeros(0)
+    near(got[:n_tok], want, lp_tol(x[:n_tok], V)[0] if n_tok else np.zeros(0))
+    assert (got[n_tok:] == 7.0).all() and errs() == (32 if n_tok > 2 else 0)
+
+
+def test_logprobs_many_tokens_of_few_rows(cuda_ok):
+    """More tokens than a row's threads, some of them twice."""
+    r = np.random.default_rng(6)
+    x = (r.standard_normal((3, 40000)) * 2).astype(np.float32)
+    tok_row, tok = r.integers(0, 3, 5000), r.integers(0, 40000, 5000)
+    tok_row[100:200], tok[100:200] = 1, 17
+    got = check_lp(x, tok_row, tok, 2)
+    assert len(set(u32(got[0][100:200]).tolist())) == 1
+
+
+def test_logprobs_and_moves_streams_and_graphs(cuda_ok):
+    """Two streams at once, then two captured graphs of attention, scoring and the move, replayed at once; the
+    graphs read what their buffers hold at each replay."""
+    L = spb200.load()
+    r = np.random.default_rng(12)
+    jobs = []
+    for i in range(2):
+        n, V = 9 + i, 33000 + 7 * i
+        c = Case(51 + i, 2, 2, 64, 32, [150 + 60 * i], [[-1] + list(range(n - 1))], layers=2, layer=1).upload()
+        x = (r.standard_normal((n, V)) * 3).astype(np.float32)
+        path = [0, 2, 3, 6, 8]
+        j = dict(c=c, x=x, V=V, n=n, d=dev(x), tok=dev(np.arange(n, dtype=np.int32)), p0=dev(np.array([0, 5], np.int32)),
+                 p=dev(np.array(path, np.int32)), lp=torch.zeros(n, device="cuda"), e=torch.zeros(n, device="cuda"),
+                 ids=torch.zeros((n, 6), dtype=torch.int32, device="cuda"), best=torch.zeros((n, 6), device="cuda"),
+                 out=torch.zeros((n, 256), device="cuda"), st=torch.cuda.Stream(), path=path)
+        jobs.append(j)
+
+    def score(j, st):
+        spb200.logprobs(j["d"].data_ptr(), j["n"], j["V"], j["V"], None, j["tok"].data_ptr(), j["n"], j["lp"].data_ptr(), None,
+                        j["e"].data_ptr(), 6, j["ids"].data_ptr(), j["best"].data_ptr(), st)
+
+    def check(j):
+        w = lp_ref(j["x"], range(j["n"]), range(j["n"]), 6)
+        t, te = lp_tol(j["x"], j["V"])
+        near(j["lp"].cpu().numpy(), w[0], t)
+        near(j["e"].cpu().numpy(), w[2], te)
+        assert np.array_equal(j["ids"].cpu().numpy(), w[3])
+        near(j["best"].cpu().numpy(), w[4], t)
+
+    for j in jobs:
+        score(j, None)
+        j["c"].run(out=j["out"])
+        j["want"] = j["out"].cpu().numpy()
+        check(j)
+        j["ids"].zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for j in jobs:
+            score(j, j["st"].cuda_stream)
+    torch.cuda.synchronize()
+    graphs = []
+    for j in jobs:
+        check(j)
+        s, c, g = j["st"].cuda_stream, j["c"], C.c_void_p()
+        j["out"].zero_()
+        torch.cuda.synchronize()
+        spb200.check(L.spb_graph_begin(s))
+        c.run(out=j["out"], stream=s)
+        score(j, s)
+        spb200.kv_compact(c.view, 1, c.d["ctx"].data_ptr(), j["p0"].data_ptr(), j["p"].data_ptr(), 5, s)
+        spb200.check(L.spb_graph_end(s, C.byref(g)))
+        graphs.append(g)
+    for rep in range(2):
+        if rep:   # other inputs in the same buffers
+            for j in jobs:
+                j["x"] = j["x"][::-1].copy()
+                j["d"].copy_(dev(j["x"]))
+                j["c"].d["k"].copy_(dev(j["c"].k))
+                j["c"].d["v"].copy_(dev(j["c"].v))
+            torch.cuda.synchronize()
+        for j, g in zip(jobs, graphs):
+            spb200.check(L.spb_graph_launch(g, j["st"].cuda_stream))
+        torch.cuda.synchronize()
+        for j in jobs:
+            check(j)
+            assert np.array_equal(u32(j["out"].cpu().numpy()), u32(j["want"]))
+            c = j["c"]
+            wk = c.k.copy()
+            for i, p in enumerate(j["path"]):
+                a, b = c.ctx[0] + p, c.ctx[0] + i
+                wk[c.tab[0, b // 32], :, :, b % 32] = wk[c.tab[0, a // 32], :, :, a % 32]
+            assert np.array_equal(c.d["k"].cpu().numpy(), wk)
+    for g in graphs:
+        L.spb_graph_free(g)
+
+
+@pytest.mark.parametrize("B", [33, 70])
+def test_attention_and_moves_of_many_sequences(cuda_ok, B):
+    """More sequences than a warp's lanes, some without nodes, in a padded batch whose last rows belong to none."""
+    r = np.random.default_rng(B)
+    ctx = [int(x) for x in r.integers(0, 90, B)]
+    trees = [tree(r, int(n)) for n in r.integers(0, 5, B)]
+    trees[0] = trees[B - 1] = []
+    c = Case(61, 1, 3, 64, 16, ctx, trees).upload()
+    want, rows = c.want(win=20), c.rows
+    c.d["q"] = torch.cat([c.d["q"], torch.full((6, 192), 1 << 23, dtype=torch.int32, device="cuda")])
+    c.d["parent"] = torch.cat([c.d["parent"], torch.full((6,), 99, dtype=torch.int32, device="cuda")])
+    c.rows = rows + 6
+    errs()
+    got = c.run(win=20).cpu().numpy()
+    assert np.array_equal(u32(got[:rows]), u32(want)) and (got[rows:] == 7.0).all() and errs() == 0
+    paths = [list(range(len(t)))[len(t) % 2:] for t in trees]   # every other one shifts by one
+    p0, p = dev(np.cumsum([0] + [len(x) for x in paths]).astype(np.int32)), dev(np.array(sum(paths, []), np.int32))
+    spb200.kv_compact(c.view, B, c.d["ctx"].data_ptr(), p0.data_ptr(), p.data_ptr(), p.numel())
+    wk = c.k.copy()
+    for b, q in enumerate(paths):
+        for i, n in enumerate(q):
+            s, t = ctx[b] + n, ctx[b] + i
+            wk[c.tab[b, t // 16], :, :, t % 16] = wk[c.tab[b, s // 16], :, :, s % 16]
+    assert np.array_equal(c.d["k"].cpu().numpy(), wk) and errs() == 0
+
+
+@pytest.mark.parametrize("G,HD,win", [(3, 64, 7), (5, 128, 40), (6, 64, 1), (7, 64, 100), (8, 128, 33)])
+def test_attention_tiles_inside_a_nodes_heads(cuda_ok, G, HD, win):
+    """16 query vectors begin inside a node's heads; windows shorter and longer than the tree is deep."""
+    c = Case(71, 2, G, HD, 24, [61], [tree(np.random.default_rng(G), 23, 0.8)]).upload()
+    assert np.array_equal(u32(c.run(win=win).cpu().numpy()), u32(c.want(win=win)))
+
+
 def test_odd_addresses_are_refused(cuda_ok):
     """Device pointers off a 4-byte boundary come back as an error (the host refuses them: nothing runs)."""
     c = Case(9, 1, 1, 64, 16, [20], [[-1, 0]]).upload()

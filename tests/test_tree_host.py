@@ -67,6 +67,14 @@ def test_logprob_refusals(args):
     assert rc(spb200.logprobs, *d.values()) == BAD
 
 
+@pytest.mark.parametrize("args", [dict(vocab=(1 << 22) + 1, ld=1 << 23), dict(rows=(1 << 26) + 1), dict(n_tok=(1 << 26) + 1),
+                                  dict(n_tok=(1 << 31) - 1)])
+def test_logprob_limits(args):
+    d = dict(logits=256, rows=4, vocab=8, ld=8, tok_row=256, tok=256, n_tok=2, logprob=256, lse=256, entropy=256, top=0, top_id=256,
+             top_logprob=256) | args
+    assert rc(spb200.logprobs, *d.values()) == UNS
+
+
 def test_nothing_to_do():
     assert rc(spb200.logprobs, None, 0, 8, 8, None, None, 0, None, None, None, 0, None, None) == 0
 
