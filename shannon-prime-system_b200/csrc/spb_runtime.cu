@@ -950,6 +950,38 @@ static bool rope_fused_enabled() {
   return on != 0;
 }
 
+// The output norm and LM head of n (at most LG_MAX) rows of the last enqueue_rows, from row r0 on: logits
+// rows [0, n) and their argmaxes
+static cudaError_t enqueue_head(spb_session *s, int r0, int n) {
+  spb_model *m = s->m;
+  cudaStream_t st = s->st;
+  cudaError_t e;
+#define K(x)                        \
+  do {                              \
+    e = (x);                        \
+    if (e != cudaSuccess) return e; \
+  } while (0)
+  const DevLayer &p = m->layers[m->NL - 1];
+  const size_t at = (size_t)r0 * m->E;
+  K(launch_norm(s->x + at, s->dn + at, m->gemma ? p.post_ffw : nullptr, m->out_norm, m->E, n, s->act, nullptr, s->err_dev,
+                st));
+  if (!m->tp) {
+    K(launch_gemv(m->out, nullptr, s->act, n, s->logits, m->V, EPI_STORE, s->err_dev, st, 0, nullptr, s->amax_keys));
+  } else {   // vocabulary rows [vbase, vbase + V): global argmax keys, then every rank's slice
+    K(launch_gemv(m->out, nullptr, s->act, n, s->logits_l, m->V, EPI_STORE, s->err_dev, st, 0, nullptr, s->amax_keys));
+    K(launch_keys_rebase(s->amax_keys, n, m->vbase, st));
+    K(tp_max_u64(m->tp, s->amax_keys, n, st, s->err_dev));
+    K(tp_gather_f32(m->tp, s->logits_l, s->logits_g, (size_t)n * m->V, st));
+    const int world = spb_tp_world(m->tp);
+    for (int r = 0; r < world; r++)   // [rank][t][V] -> [t][rank * V + j]
+      K(cudaMemcpy2DAsync(s->logits + (size_t)r * m->V, (size_t)m->Vfull * 4, s->logits_g + (size_t)r * n * m->V,
+                          (size_t)m->V * 4, (size_t)m->V * 4, n, cudaMemcpyDeviceToDevice, st));
+  }
+  K(launch_argmax_take(s->amax_keys, n, s->argmax_dev, st));
+#undef K
+  return cudaSuccess;
+}
+
 // Enqueue the schedule for nt rows (tokens already in tok_dev, positions at pos_dev). With
 // rows (device, [nt]), row t belongs to its own session: RoPE/KV store and attention use that
 // session's cache and position; Pmax is the largest of their capacities. With n_trees, the rows
@@ -1034,26 +1066,7 @@ static cudaError_t enqueue_rows(spb_session *s, int nt, bool want_logits, const 
     K(launch_quant(s->gg, m->FF, m->FF, nt, s->act, s->gg_max, s->err_dev, st));
     K(split_gemv(d.d, s->dn));
   }
-  if (want_logits) {
-    const DevLayer &p = m->layers[m->NL - 1];
-    K(launch_norm(s->x, s->dn, m->gemma ? p.post_ffw : nullptr, m->out_norm, E, nt, s->act, nullptr, s->err_dev, st));
-    if (!m->tp) {
-      K(launch_gemv(m->out, nullptr, s->act, nt, s->logits, m->V, EPI_STORE, s->err_dev, st, 0, nullptr,
-                    s->amax_keys));
-    } else {   // vocabulary rows [vbase, vbase + V): global argmax keys, then every rank's slice
-      K(launch_gemv(m->out, nullptr, s->act, nt, s->logits_l, m->V, EPI_STORE, s->err_dev, st, 0, nullptr,
-                    s->amax_keys));
-      K(launch_keys_rebase(s->amax_keys, nt, m->vbase, st));
-      K(tp_max_u64(m->tp, s->amax_keys, nt, st, s->err_dev));
-      K(tp_gather_f32(m->tp, s->logits_l, s->logits_g, (size_t)nt * m->V, st));
-      const int world = spb_tp_world(m->tp);
-      for (int r = 0; r < world; r++)   // [rank][t][V] -> [t][rank * V + j]
-        K(cudaMemcpy2DAsync(s->logits + (size_t)r * m->V, (size_t)m->Vfull * 4,
-                            s->logits_g + (size_t)r * nt * m->V, (size_t)m->V * 4, (size_t)m->V * 4, nt,
-                            cudaMemcpyDeviceToDevice, st));
-    }
-    K(launch_argmax_take(s->amax_keys, nt, s->argmax_dev, st));
-  }
+  if (want_logits) K(enqueue_head(s, 0, nt));
 #undef K
   return cudaSuccess;
 }
@@ -1243,23 +1256,27 @@ extern "C" int spb_session_score(spb_session *s, const int32_t *tokens, int n_to
   if (!rc) rc = sync_pos(s);
   if (rc) return rc;
   if (out->logprob) out->logprob[0] = NAN;   // its predecessor's row belongs to an earlier call
-  for (int done = 0; done < n_tok;) {
-    int nt = LG_MAX;
+  for (int done = 0; done < n_tok;) {   // the layers in prefill's chunks, the LM head LG_MAX rows at a time
+    int nt = NT_MAX;
     while (nt > n_tok - done) nt >>= 1;
     memcpy(s->h_pinned, tokens + done, (size_t)nt * 4);
     CU(cudaMemcpyAsync(s->tok_dev, s->h_pinned, (size_t)nt * 4, cudaMemcpyHostToDevice, s->st));
-    const int nlp = std::min(nt, n_tok - done - 1);   // row t against the token that follows it
-    for (int t = 0; t < nlp; t++) {
-      s->h_nodes[LG_MAX + t] = t;
-      s->h_nodes[2 * LG_MAX + t] = tokens[done + t + 1];
-    }
-    CU(cudaMemcpyAsync(s->nodes_dev + LG_MAX, s->h_nodes + LG_MAX, (size_t)2 * LG_MAX * 4, cudaMemcpyHostToDevice,
-                       s->st));
-    CU(enqueue_rows(s, nt, true));
+    CU(enqueue_rows(s, nt, false));
     CU(launch_advance(s->pos_dev, nt, nullptr, nullptr, s->st));
-    rc = emit_out(s, nt, done, nlp, done + 1, out);
-    if (rc) return rc;
-    CU(cudaStreamSynchronize(s->st));   // the staging is written again by the next chunk
+    for (int r0 = 0; r0 < nt; r0 += LG_MAX) {
+      const int n = std::min(LG_MAX, nt - r0), first = done + r0;
+      const int nlp = std::min(n, n_tok - first - 1);   // row t against the token that follows it
+      for (int t = 0; t < nlp; t++) {
+        s->h_nodes[LG_MAX + t] = t;
+        s->h_nodes[2 * LG_MAX + t] = tokens[first + t + 1];
+      }
+      CU(cudaMemcpyAsync(s->nodes_dev + LG_MAX, s->h_nodes + LG_MAX, (size_t)2 * LG_MAX * 4, cudaMemcpyHostToDevice,
+                         s->st));
+      CU(enqueue_head(s, r0, n));
+      rc = emit_out(s, n, first, nlp, first + 1, out);
+      if (rc) return rc;
+      CU(cudaStreamSynchronize(s->st));   // the staging is written again by the next rows
+    }
     done += nt;
   }
   rc = collect_errors(s);

@@ -854,3 +854,28 @@ def test_score(xr, cuda_ok, env, n):
     assert np.array_equal(u32(s.step(3)), u32(xs.step(3)))
     s.close()
     xs.close()
+
+
+def test_score_long_and_in_pieces(xr, cuda_ok, env):
+    """A whole chunk of 256 rows and its rest; pieces give the bytes of the whole, but for their first tokens."""
+    cfg, T, m, pool = env
+    n = 323
+    s, xs = m.session(400), xr.session(xref.build_desc(cfg, T), 400)
+    toks = spmodel.gen_tokens(43, n, cfg.n_vocab)
+    res, rows = s.score(toks, top=3, logits=True), xs.prefill(toks)
+    assert np.array_equal(u32(res.logits), u32(rows)) and s.position() == n
+    tol, tol_e = lp_tol(rows, cfg.n_vocab)
+    lp, _, ent, ids, best = lp_ref(rows, range(n - 1), toks[1:], 3)
+    near(res.logprob[1:], lp, tol[:-1])
+    near(res.entropy, ent, tol_e)
+    assert np.array_equal(res.top_id, ids) and np.array_equal(res.argmax, rows.argmax(1))
+    near(res.top_logprob, best, tol)
+    s.rewind(n)
+    at = 0
+    for k in (1, 130, n - 131):
+        part = s.score(toks[at:at + k], top=3)
+        assert np.isnan(part.logprob[0]) and np.array_equal(u32(part.logprob[1:]), u32(res.logprob[at + 1:at + k]))
+        assert np.array_equal(u32(part.entropy), u32(res.entropy[at:at + k])) and np.array_equal(part.top_id, res.top_id[at:at + k])
+        at += k
+    s.close()
+    xs.close()
