@@ -6,9 +6,10 @@
 // finite or +inf entry has lse -inf and entropy 0; a row that holds NaN or +inf has no
 // distribution: lse, entropy, its tokens' logprobs and its alternatives' are NaN, the ids -1.
 //
-// One pass over the logits, so memory bounds it. A row is cut into up to 16 parts of at least 16384 entries;
-// a CTA's thread takes every 512th group of four neighbours of a part, a warp joins its threads' sums, and a
-// part its sixteen warps'. A cluster of C CTAs shares the parts of a row; C follows from the rows of the
+// One pass over the logits, so memory bounds it: 1000 rows x 151936 take 109 us, 85 % of the measured copy
+// rate; 64 rows x 262144 16.5 us (62 %: 256 CTAs do not divide 148 SMs evenly), 23.9 with 20 alternatives. A
+// row is cut into up to 16 parts of at least 16384 entries; a CTA's thread takes every 512th group of four
+// neighbours of a part, a warp joins its threads' sums, and a part its sixteen warps'. A cluster of C CTAs shares the parts of a row; C follows from the rows of the
 // call (few rows: a row over many CTAs), but what is summed in which order follows from the vocabulary's
 // size alone, so a row's bytes depend neither on the other rows nor on its alignment.
 //
@@ -411,8 +412,8 @@ cudaError_t launch_logprobs(const LogprobArgs &a, cudaStream_t st) {
   const int per = ((a.vocab + P - 1) / P + 3) & ~3;
   P = (a.vocab + per - 1) / per;
   // few rows: a row over as many CTAs as it has parts; more: over fewer, so that the call is one wave of two
-  // CTAs per SM (64 rows x 262144, 20 alternatives: 45 us with at most one per SM, 29 with two, 43 and 61
-  // with two and four waves); many rows: a CTA each, three per SM
+  // CTAs per SM (64 rows x 262144, 20 alternatives, at that step: 45 us with at most one per SM, 29 with two,
+  // 43 and 61 with two and four waves); many rows: a CTA each, three per SM
   int C = P;
   if ((long long)a.rows * C > 2 * 148) C = a.rows < 2 * 148 ? 2 * 148 / a.rows : 1;
   const int each = (P + C - 1) / C;   // parts of a CTA, spread evenly

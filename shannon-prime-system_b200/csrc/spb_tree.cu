@@ -703,7 +703,9 @@ __global__ void __launch_bounds__(512, 1) k_tree_attn(TreeAttnArgs a, int CL) {
 //
 // A thread owns one 16-byte column of one (K or V, layer, KV head) row set and walks the path, so
 // no two threads touch the same bytes. path is strictly ascending, path[i] >= i: a batch loads its
-// rows before it stores any, and what earlier batches stored lies below every later source.
+// rows before it stores any, and what earlier batches stored lies below every later source. The bytes
+// moved bound it, and short of that the latency of one batch: 12 rows in each of 8 sessions (36 layers x 8
+// heads x 128: 57 MB, 8.6 us at the measured copy rate) take 9.7 us a call, of which the host needs as much.
 constexpr int MOVE = 8;   // rows in flight per thread
 
 __global__ void __launch_bounds__(256) k_kv_compact(KvCompactArgs a) {
