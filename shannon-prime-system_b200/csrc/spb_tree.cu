@@ -166,7 +166,9 @@ __device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
 // cycle. Measured and not kept (64 nodes at context 8192, 217 us): 32 query vectors per CTA (364: the sums
 // spill, V comes in pieces of 32 bytes), 8 warps of twice the dims (241), V through shared memory for the
 // whole CTA (260: a barrier per step) or in a ring per warp (229: 80 KB that the L1 misses while K comes
-// in), a row's pieces fetched by neighbouring lanes and shuffled (214, small trees 2 to 4 % slower).
+// in), a row's pieces fetched by neighbouring lanes and shuffled (214, small trees 2 to 4 % slower), 16 slots
+// per warp and step of K, which halves the reads of the queries' planes but takes 128 bytes of a row at a time
+// (262).
 // MULTI (more slots per rank than scores are kept for): the maxima first, then scores again in runs of
 // CS slots, each run's V-sums added up in shared memory.
 template <int HD, bool MULTI>
