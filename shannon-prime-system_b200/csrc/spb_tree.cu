@@ -156,19 +156,21 @@ __device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
 //   scores    a warp takes 8 slots at a time: their K rows go from global memory straight into the
 //             column operand (a lane's 32 bytes are eight columns of one slot, so the digit planes
 //             are a byte transpose in registers), the queries' planes wait in shared memory;
-//             9 products, 32 cycles a slot at HD 256 (18 of them the matrix units')
+//             9 products, 33 cycles a slot at HD 256 (18 of them the matrix units', 6 the recombination
+//             and scaling of its eight slots; without the K loads as long)
 //   exps      in place over the scores, each four neighbours' bytes transposed into the planes of
 //             the row operand; 7 cycles a slot
 //   V-sums    a warp takes 16 head dims over the slots of the run, V rows again straight from global
-//             memory (eight slots x two dims per lane and step); 12 products, 46 cycles a slot (24 the
-//             matrix units')
-// Both passes wait for memory: an SM has 64 KB of rows on their way and gets 32 (K) and 23 (V) bytes a
-// cycle. Measured and not kept (64 nodes at context 8192, 217 us): 32 query vectors per CTA (364: the sums
+//             memory (eight slots x two dims per lane and step); 12 products, 50 cycles a slot (24 the
+//             matrix units'; 36 if the same bytes lay in 256-byte pieces: 64 bytes of a row at a time cost
+//             the L1 its lookups, as much when every one of them hits)
+// and 28000 cycles a CTA besides: finding the tile 2600, rows 2400, queries and parents 5500, the maxima's
+// exchange 5000, the sums' 9500, the division 2600 (2080 slots; a cluster of 4).
+// Measured and not kept (64 nodes at context 8192, 217 us): 32 query vectors per CTA (364: the sums
 // spill, V comes in pieces of 32 bytes), 8 warps of twice the dims (241), V through shared memory for the
 // whole CTA (260: a barrier per step) or in a ring per warp (229: 80 KB that the L1 misses while K comes
 // in), a row's pieces fetched by neighbouring lanes and shuffled (214, small trees 2 to 4 % slower), 16 slots
-// per warp and step of K, which halves the reads of the queries' planes but takes 128 bytes of a row at a time
-// (262).
+// per warp and step of K (262), K in runs of four steps, in two buffers (spills) or in one (217 both).
 // MULTI (more slots per rank than scores are kept for): the maxima first, then scores again in runs of
 // CS slots, each run's V-sums added up in shared memory.
 template <int HD, bool MULTI>
