@@ -169,8 +169,9 @@ __device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
 // Measured and not kept (64 nodes at context 8192, 217 us): 32 query vectors per CTA (364: the sums
 // spill, V comes in pieces of 32 bytes), 8 warps of twice the dims (241), V through shared memory for the
 // whole CTA (260: a barrier per step) or in a ring per warp (229: 80 KB that the L1 misses while K comes
-// in), a row's pieces fetched by neighbouring lanes and shuffled (214, small trees 2 to 4 % slower), 16 slots
-// per warp and step of K (262), K in runs of four steps, in two buffers (spills) or in one (217 both).
+// in), a row's pieces fetched by neighbouring lanes and shuffled (214, small trees 2 to 4 % slower), whole lines
+// of V by two neighbouring warps that hand each other their planes (290: a barrier per step), 16 slots per warp
+// and step of K (262), K in runs of four steps, in two buffers (spills) or in one (217 both).
 // MULTI (more slots per rank than scores are kept for): the maxima first, then scores again in runs of
 // CS slots, each run's V-sums added up in shared memory.
 template <int HD, bool MULTI>
