@@ -258,7 +258,7 @@ typedef struct {
  * rows are in slot ctx[s] + i already, its position is ctx[s] + its depth. q and out [rows][n_head
  * head_dim]: rotated queries on the 2^16 grid (|q| < 2^24), f32 outputs. window <= 0: none, else a
  * node sees the window positions up to its own. max_ctx (host): no ctx[s] is larger; it, or the window
- * where that is shorter, is at most 1048512 (SPB_EUNSUPPORTED). ctx, row0
+ * where that is shorter, is at most 1048512, and max_ctx itself at most 2^30 (SPB_EUNSUPPORTED). ctx, row0
  * [n_seq + 1], parent, q, out and the view's pointers are memory of the current device; nothing is
  * allocated after the first call on a device, calls on different streams are independent. A sequence
  * whose arrays are out of range raises a bit (spb_take_device_errors) and leaves its rows as they

@@ -1840,6 +1840,7 @@ extern "C" int spb_tree_attn(const spb_kv_view *kv, int layer, int n_seq, const 
     return set_err(SPB_EUNSUPPORTED, "spb_tree_attn: n_head/n_head_kv must be an integer <= 8");
   if ((window > 0 ? std::min(window, max_ctx) : max_ctx) > TREE_SPAN - TREE_NODES)
     return set_err(SPB_EUNSUPPORTED, "spb_tree_attn: %d visible positions at most", TREE_SPAN - TREE_NODES);
+  if (max_ctx > (1 << 30)) return set_err(SPB_EUNSUPPORTED, "spb_tree_attn: contexts of 2^30 positions at most");
   if (rows == 0) return SPB_OK;
   if (!ctx || !row0 || !parent || !q || !out) return set_err(SPB_EBADARG, "spb_tree_attn: null arg");
   if ((uintptr_t)q & 15) return set_err(SPB_EBADARG, "spb_tree_attn: q must be 16-byte aligned");

@@ -67,6 +67,12 @@ def test_logprob_refusals(args):
     assert rc(spb200.logprobs, *d.values()) == BAD
 
 
+@pytest.mark.parametrize("max_ctx,window,code", [(1048513, -1, UNS), (1 << 29, 1048513, UNS), ((1 << 30) + 1, 1024, UNS),
+                                                 ((1 << 31) - 1, 64, UNS), (1 << 30, 1024, BAD)])   # (the last: only its pointers are bad)
+def test_attention_limits(max_ctx, window, code):
+    assert rc(spb200.tree_attn, view(), 0, 2, 256, 256, 256, 2, max_ctx, 256, 4, window, 256) == code
+
+
 @pytest.mark.parametrize("args", [dict(vocab=(1 << 22) + 1, ld=1 << 23), dict(rows=(1 << 26) + 1), dict(n_tok=(1 << 26) + 1),
                                   dict(n_tok=(1 << 31) - 1)])
 def test_logprob_limits(args):
