@@ -638,6 +638,26 @@ def test_attention_and_moves_of_many_sequences(cuda_ok, B):
     assert np.array_equal(c.d["k"].cpu().numpy(), wk) and errs() == 0
 
 
+def test_attention_far_positions(cuda_ok):
+    """A window behind 2^29 and 2^30 - 70 positions of a page table that names two pages again and again."""
+    page, n, win = 8192, 9, 300
+    c = Case(81, 2, 2, 64, page, [page - n, page - n], [tree(np.random.default_rng(4), n)] * 2, spare=0).upload()
+    ctx = [(1 << 29) + 77, (1 << 30) - 70]
+    tab = torch.zeros((2, (1 << 30) // page), dtype=torch.int32, device="cuda")
+    tab[0, 0::2], tab[0, 1::2] = int(c.tab[0, 0]), int(c.tab[1, 0])
+    tab[1, 0::2], tab[1, 1::2] = int(c.tab[1, 0]), int(c.tab[0, 0])
+    c.d["ctx"], c.view.ptab, c.view.ptab_ld = dev(np.array(ctx, np.int32)), tab.data_ptr(), tab.shape[1]
+    errs()
+    got = c.run(win=win, max_ctx=1 << 30).cpu().numpy()
+    assert errs() == 0
+    want = []
+    for b in range(2):
+        slots = np.arange(ctx[b] - win, ctx[b] + n)   # nothing before them is visible
+        pg = tab[b].cpu().numpy()[slots // page]
+        want.append(attend(c.k[pg, 0, :, slots % page], c.v[pg, 0, :, slots % page], c.q[n * b:n * b + n], win, c.trees[b], win, 2))
+    assert np.array_equal(u32(got), u32(np.concatenate(want)))
+
+
 @pytest.mark.parametrize("G,HD,win", [(3, 64, 7), (5, 128, 40), (6, 64, 1), (7, 64, 100), (8, 128, 33)])
 def test_attention_tiles_inside_a_nodes_heads(cuda_ok, G, HD, win):
     """16 query vectors begin inside a node's heads; windows shorter and longer than the tree is deep."""
