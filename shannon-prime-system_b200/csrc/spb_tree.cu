@@ -117,8 +117,8 @@ constexpr int32_t UNSEEN = INT32_MIN;   // the score of a position that a node d
 
 // exp_fixed of a score's distance below its maximum in 32-bit steps: far = max - z in units of 2^-14,
 // g = ceil(far log2(e)) in 2^30, n = g >> 30 octaves and the rest; the island's polynomial in x = 2^30 -
-// rest, each (acc x) >> 30 as the high word of acc * 4x (x < 2^30 here). 363410 steps are 32 octaves, the
-// island's zero.
+// rest, each (acc x) >> 30 as the high word of acc * 4x (x < 2^30 here). 32 octaves (363408.75 steps) and
+// more are the island's zero.
 __device__ __forceinline__ uint32_t mad_hi(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("mad.hi.u32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -135,7 +135,7 @@ __device__ __forceinline__ uint32_t exp_grid(int32_t z, int32_t mx) {
   acc = mad_hi(acc, x4, 744261118u);
   acc = mad_hi(acc, x4, 1073741824u) >> 1;
   acc = (r4 == 0u ? 1u << 30 : acc) >> (n & 31u);
-  return z == UNSEEN || far >= 363410u ? 0u : acc;
+  return z == UNSEEN || n >= 32u ? 0u : acc;
 }
 
 // f32 of floor(N 2^16 / S) 2^-32 (the decode attention's rounding), r = 2^16 / S in double: N r is off by
