@@ -13,9 +13,10 @@
 // call (few rows: a row over many CTAs), but what is summed in which order follows from the vocabulary's
 // size alone, so a row's bytes depend neither on the other rows nor on its alignment.
 //
-// A thread sums e^(x - m) = 2^(x L - M), L = log2(e) in f32 and M = m L rounded, for a reference m that is
-// its first groups' maximum and moves only when entries are more than 2^RISE above it; the weighted sum
-// takes the same exponents. L's rounding scales every entry by 1 + 1.3e-8, M's is taken off at the end.
+// A thread sums e^(x - m) = 2^((x - m) L), L = log2(e) in f32, for a reference m that is its first groups'
+// maximum and moves only when entries are more than RISE above it; the weighted sum takes the same exponents.
+// The difference comes first: in x L - m L the rounding of m L grows with m (0.5 at 1e7, 2^99 at 1e37) and would
+// stand in the exponent.
 //
 // The largest entries: the top'th largest of the threads' maxima bounds the top'th largest entry from below,
 // and only the threads that reach it can hold larger ones: their groups are read again (from L2) and what
@@ -114,30 +115,18 @@ __device__ __forceinline__ void part(const float *x, int p0, int p1, int vocab, 
       r.s = __fmul_rn(r.s, f);
       r.m = bm;
     }
-    const float m = r.m == -INFINITY ? 0.0f : r.m, M = __fmul_rn(m, LOG2E_F);
-    if (fabsf(m) < 1e37f) {
-      float s = 0.0f, t = 0.0f;
+    const float m = r.m == -INFINITY ? 0.0f : r.m;
+    float s = 0.0f, t = 0.0f;
 #pragma unroll
-      for (int u = 0; u < LBATCH; u++)
+    for (int u = 0; u < LBATCH; u++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float a = max_nan(__fmaf_rn(v[u][i], LOG2E_F, -M), FLOOR2), e = exp2_fast(a);
-          s = __fadd_rn(s, e);
-          if (ENT) t = __fmaf_rn(e, a, t);
-        }
-      const float d = __fmaf_rn(m, LOG2E_F, -M);   // M's rounding, exactly: 2^-d = 1 - d ln 2
-      r.t = __fadd_rn(r.t, __fmaf_rn(-d, __fmaf_rn(0.693147182f, t, s), t));
-      r.s = __fadd_rn(r.s, __fmaf_rn(__fmul_rn(-d, 0.693147182f), s, s));
-    } else {   // (m L may overflow)
-#pragma unroll
-      for (int u = 0; u < LBATCH; u++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float a = max_nan(__fmul_rn(__fsub_rn(v[u][i], m), LOG2E_F), FLOOR2), e = exp2_fast(a);
-          r.s = __fadd_rn(r.s, e);
-          r.t = __fmaf_rn(e, a, r.t);
-        }
-    }
+      for (int i = 0; i < 4; i++) {
+        const float a = max_nan(__fmul_rn(__fsub_rn(v[u][i], m), LOG2E_F), FLOOR2), e = exp2_fast(a);
+        s = __fadd_rn(s, e);
+        if (ENT) t = __fmaf_rn(e, a, t);
+      }
+    r.s = __fadd_rn(r.s, s);
+    r.t = __fadd_rn(r.t, t);
   }
 }
 

@@ -1,15 +1,16 @@
 """Values at which the kernels that verify drafted trees can go wrong: every distance of a score below
-its maximum."""
+its maximum, logits of every magnitude, finite masks."""
 import numpy as np
 import pytest
 import torch
 
 import spb200
-from test_gpu_tree import dev, errs, exp_fixed, u32
+from test_gpu_tree import dev, errs, exp_fixed, run_lp, u32
 
 pytestmark = pytest.mark.gpu
 
 ONE = 1 << 30
+U = 2.0 ** -24                                             # half a step of f32, relative
 
 
 # ------------------------------------------------------------------------------ attention
@@ -39,3 +40,100 @@ def test_attention_every_distance_below_the_maximum(cuda_ok):
     want = (((w // S) << 16) + ((w % S) << 16) // S).astype(np.float64) * 2.0 ** -32
     wrong = (u32(got) != u32(want.astype(np.float32))).any(1)
     assert not wrong.any(), far[wrong]
+
+
+# ------------------------------------------------------------------------------ log probabilities
+def lp_exact(x, tok_row, tok, top):
+    """64-bit, from differences to the row's maximum (x - lse would lose log(sum) to a maximum of 1e30)."""
+    x = x.astype(np.float64)
+    m = x.max(1, keepdims=True)
+    d = np.maximum(x - m, -1e300)
+    e = np.exp(d)
+    s = e.sum(1)
+    mean = (e * np.where(e > 0, d, 0.0)).sum(1) / s        # sum p (x - m)
+    order = np.argsort(-x, axis=1, kind="stable")[:, :top]
+    at = np.take_along_axis(x, order, 1)
+    ids = np.where(at > -np.inf, order, -1)
+    best = at - m - np.log(s)[:, None]
+    lp = (x[tok_row, tok] - m[tok_row, 0]) - np.log(s)[tok_row]
+    low = -3.4028236e38                                    # differences below f32's lowest value have no f32 but -inf
+    return np.where(lp < low, -np.inf, lp), m[:, 0] + np.log(s), np.log(s) - mean, ids, np.where(best < low, -np.inf, best)
+
+
+def lp_bounds(x):
+    """How far log(sum), and the entropy, may be off; every rounding at most U of its value.
+
+    An addend e = 2^((x - r) log2 e) of a thread's reference r: the exponential 4 U, its argument two roundings
+    and the constant's (2.25 U |x - r|). Sums are moved to larger references at most N times (a thread's batches
+    of 8192 entries, the warp, 16 warps by halves, 16 parts by halves): 4 U for the factor, 3 U for its use,
+    U of the distance; the largest entry's own reference is the row's maximum: factors of 1, no error. Additions: as
+    many as there are other entries above -inf, at most 16 in a batch, one a batch, 5 in the warp and the halvings'.
+    The entropy's second sum has the same terms times their distance D (of one sign), a product and a shift of
+    its own at every step."""
+    x = x.astype(np.float64)
+    m = x.max(1, keepdims=True)
+    d = np.maximum(x - m, -1e300)
+    e = np.exp(d)
+    S = e.sum(1)
+    p, D = e / S[:, None], np.where(e > 0, -d, 0.0)
+    mean, sq = (p * D).sum(1), (p * D * D).sum(1)
+    V = x.shape[1]
+    parts = min(16, -(-V // 16384))
+    batches = -(-(-(-V // parts) + 3) // 8192)
+    N = batches + 10
+    A = np.minimum(30 + batches, (x > -np.inf).sum(1) - 1)
+    rel = (1 - p.max(1)) * (4 + 7 * N) + 3.25 * mean + A
+    log = U * (rel + 2 * np.log(S))                        # (logf: one unit in its last place)
+    ent = U * ((8 + 10 * N + 2 * A) * mean + 3.25 * sq + rel * mean + 4 * mean + 2 * (np.log(S) + mean))
+    return log * 1.01 + 1e-38, (log + ent) * 1.01 + 1e-38  # (products of two errors)
+
+
+def off(got, want, tol):
+    f = np.isfinite(want)
+    assert np.array_equal(got[~f], want[~f]), (got[~f], want[~f])
+    d = np.abs(got[f].astype(np.float64) - want[f]) - np.broadcast_to(tol, want.shape)[f]
+    assert (d <= 0).all(), (d.max(), np.argwhere(f)[d.argmax()], got[f][d.argmax()], want[f][d.argmax()])
+
+
+def check_rows(x, tok, top=5, **kw):
+    """Every row's log-sum-exp, entropy, alternatives and the log probabilities of the given columns."""
+    x = x.astype(np.float32)
+    rows = np.repeat(np.arange(len(x)), len(tok))
+    tok = np.tile(np.asarray(tok), len(x))
+    errs()
+    got, want = run_lp(x, rows, tok, top, **kw), lp_exact(x, rows, tok, top)
+    assert errs() == 0
+    log, ent = lp_bounds(x)
+    m = x.max(1).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        off(got[0], want[0], log[rows] + U * (np.abs(x[rows, tok] - m[rows]) + np.abs(want[0])))
+        off(got[1], want[1], log + U * np.abs(want[1]))
+        off(got[2], want[2], ent + U * np.abs(want[2]))
+        assert np.array_equal(got[3], want[3])
+        off(got[4], want[4], log[:, None] + U * (2 * np.abs(want[4]) + log[:, None] + np.log(len(x[0]))))
+    assert (got[2] >= 0).all()
+
+
+MASKS = [-1e4, -65504.0, -1e9, -10 ** 9.5, -1e10, -1e18, -1e20, -1e30, -1e36, float(np.finfo(np.float32).min)]
+
+
+@pytest.mark.parametrize("V", [32000, 262144])
+def test_logprobs_finite_masks(cuda_ok, V):
+    """Masks written as large negative numbers, over half of a row, most of it, and its front or tail."""
+    r = np.random.default_rng(1)
+    x = []
+    for mask in MASKS:
+        for where in (r.random(V) < 0.5, r.random(V) < 0.9, np.arange(V) < V // 2, np.arange(V) >= V // 3, np.arange(V) != 777):
+            x.append(np.where(where, mask, r.standard_normal(V) * 3))
+    check_rows(np.stack(x), [777, V // 3 - 1, V - 1, 0])
+
+
+def test_logprobs_rows_of_any_magnitude(cuda_ok):
+    """Rows of one value, and ordinary rows around a far value, at every magnitude that f32 has."""
+    V, r = 20011, np.random.default_rng(2)
+    x = [np.full(V, s * 10.0 ** k) for k in (0, 2, 3, 3.6, 4, 5, 6, 7, 7.3, 8, 9, 9.5, 10, 12, 15, 20, 25, 30, 36, 37, 38) for s in (1, -1)]
+    for c in (1e3, 4e3, 5e3, 1e4, 1e5, 1e6, 1e7, 3e7, 1e8, 1e9, 3e9):
+        x += [r.standard_normal(V) * 3 + c, r.standard_normal(V) * 3 - c]
+    for k in range(-6, 39, 2):                             # a spread of that size
+        x.append(r.uniform(-1, 1, V) * 3 * 10.0 ** k)
+    check_rows(np.stack(x), [0, 9999, V - 1], top=20)
