@@ -13,8 +13,10 @@
 // call (few rows: a row over many CTAs), but what is summed in which order follows from the vocabulary's
 // size alone, so a row's bytes depend neither on the other rows nor on its alignment.
 //
-// A thread sums e^(x - m) = 2^((x - m) L), L = log2(e) in f32, for a reference m that is its first groups'
-// maximum and moves only when entries are more than RISE above it; the weighted sum takes the same exponents.
+// A thread sums e^(x - m) = 2^((x - m) L), L = log2(e) in f32, and the same weighted by the exponents, with m
+// the largest entry it has met: so the row's largest entry counts 1 exactly, sum e >= 1, and neither log(sum e) nor
+// x - m holds digits that the other has to cancel (a reference below the maximum costs a likely token's log
+// probability and a peaked row's entropy 1e-6).
 // The difference comes first: in x L - m L the rounding of m L grows with m (0.5 at 1e7, 2^99 at 1e37) and would
 // stand in the exponent.
 //
@@ -40,8 +42,9 @@ constexpr int LPARTS = 16;
 constexpr int LCAND = 2048;        // entries at or above the bound that are ranked by counting
 constexpr int LBATCH = 4;          // groups of four in flight per thread
 constexpr float LOG2E_F = 1.44269504f;
+constexpr float LOG2E_LO = 1.92596299e-8f;   // log2(e) - LOG2E_F
+constexpr float LN2_F = 0.693147182f;
 constexpr float FLOOR2 = -200.0f;  // exponents of two below this are zero in f32
-constexpr float RISE = 16.0f;      // entries this far above the reference move it (e^16 times 2^22 entries fit f32)
 
 // larger value first, equal values lowest id first (-0 and +0 are equal); every entry above -inf is above 0
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -68,9 +71,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
 }
 
 struct Running {
-  float m, s, t;   // reference, sum of 2^((x - m) L), the same weighted by its exponent
-  float top;       // largest entry
+  float m, s, t;   // largest entry, sum of 2^((x - m) L), the same weighted by its exponent
 };
+
+// e^d, d <= 0 the distance of two references (at least one above -inf; else 0), and its exponent of two a. A
+// reference stands for many entries at once: the rounding of a and log2(e)'s rest are made good.
+__device__ __forceinline__ float rescale(float d, float &a) {
+  d = fmaxf(d, -140.0f);   // (e^-140 is zero in f32, and NaN, of equal infinities, becomes that)
+  a = __fmul_rn(d, LOG2E_F);
+  const float f = exp2_fast(a), rest = __fmaf_rn(d, LOG2E_LO, __fmaf_rn(d, LOG2E_F, -a));
+  return __fmaf_rn(f, __fmul_rn(rest, LN2_F), f);
+}
 
 // part [p0, p1) of a row that starts SH floats behind a 16-byte boundary
 template <int SH, bool ENT>
@@ -108,9 +119,9 @@ __device__ __forceinline__ void part(const float *x, int p0, int p1, int vocab, 
     for (int u = 0; u < LBATCH; u++)
 #pragma unroll
       for (int i = 0; i < 4; i++) bm = fmaxf(bm, v[u][i]);
-    r.top = fmaxf(r.top, bm);
-    if (bm > __fadd_rn(r.m, RISE)) {   // (a first finite entry, or a steep rise)
-      const float a = fmaxf(__fmul_rn(__fsub_rn(r.m, bm), LOG2E_F), FLOOR2), f = exp2_fast(a);
+    if (bm > r.m) {
+      float a;
+      const float f = rescale(__fsub_rn(r.m, bm), a);
       r.t = __fmul_rn(f, __fmaf_rn(r.s, a, r.t));
       r.s = __fmul_rn(r.s, f);
       r.m = bm;
@@ -139,9 +150,8 @@ __device__ __forceinline__ unsigned long long warp_max_u64(unsigned long long v)
 // (m, s, t) of two disjoint sets of entries as one, s and t being sums relative to m
 __device__ __forceinline__ void join(float &m, float &s, float &t, float m2, float s2, float t2) {
   const float mm = fmaxf(m, m2);
-  const float a = m == -INFINITY ? FLOOR2 : max_nan(__fmul_rn(__fsub_rn(m, mm), LOG2E_F), FLOOR2);
-  const float b = m2 == -INFINITY ? FLOOR2 : max_nan(__fmul_rn(__fsub_rn(m2, mm), LOG2E_F), FLOOR2);
-  const float f = exp2_fast(a), g = exp2_fast(b);
+  float a, b;
+  const float f = rescale(__fsub_rn(m, mm), a), g = rescale(__fsub_rn(m2, mm), b);
   t = __fadd_rn(__fmul_rn(f, __fmaf_rn(s, a, t)), __fmul_rn(g, __fmaf_rn(s2, b, t2)));
   s = __fadd_rn(__fmul_rn(s, f), __fmul_rn(s2, g));
   m = mm;
@@ -188,19 +198,20 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
 #pragma unroll 1
   for (int p = rank, i = 0; p < P; p += C, i++) {
     const int p0 = p * per, p1 = min(p0 + per, a.vocab);
-    Running r{-INFINITY, 0.0f, 0.0f, -INFINITY};
+    Running r{-INFINITY, 0.0f, 0.0f};
     switch (sh) {
       case 0: part<0, ENT>(x, p0, p1, a.vocab, r); break;
       case 1: part<1, ENT>(x, p0, p1, a.vocab, r); break;
       case 2: part<2, ENT>(x, p0, p1, a.vocab, r); break;
       default: part<3, ENT>(x, p0, p1, a.vocab, r); break;
     }
-    largest = fmaxf(largest, r.top);
+    largest = fmaxf(largest, r.m);
     float m = r.m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float d = r.m == -INFINITY ? FLOOR2 : max_nan(__fmul_rn(__fsub_rn(r.m, m), LOG2E_F), FLOOR2), f = exp2_fast(d);
-    float s = __fmul_rn(r.s, f), t = __fmul_rn(f, __fmaf_rn(r.s, d, r.t));
+    float shift;
+    const float f = rescale(__fsub_rn(r.m, m), shift);
+    float s = __fmul_rn(r.s, f), t = __fmul_rn(f, __fmaf_rn(r.s, shift, r.t));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, o));
@@ -330,12 +341,12 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
       ls_sh = ls;
       if (rank == 0) {
         if (a.lse) a.lse[row] = none ? NAN : s > 0.0f ? __fadd_rn(m, ls) : -INFINITY;
-        if (a.entropy) a.entropy[row] = none ? NAN : s > 0.0f ? __fsub_rn(ls, __fmul_rn(0.693147182f, __fdiv_rn(t, s))) : 0.0f;
+        if (a.entropy) a.entropy[row] = none ? NAN : s > 0.0f ? __fsub_rn(ls, __fmul_rn(LN2_F, __fdiv_rn(t, s))) : 0.0f;
       }
     }
   }
   __syncthreads();
-  // x - lse as (x - m) - log(s): likely tokens keep the digits that lse has lost to m
+  // x - lse as (x - m) - log(s), m the row's maximum: likely tokens keep the digits that lse has lost to m
   const float m0 = m_sh, ls = ls_sh;
   auto logprob = [&](float x) { return ls != ls ? NAN : x == -INFINITY ? -INFINITY : __fsub_rn(__fsub_rn(x, m0), ls); };
   // ---- this row's tokens: without tok_row token `row`, else every row's CTAs look through the list (row 0's

@@ -1,5 +1,5 @@
 """Values at which the kernels that verify drafted trees can go wrong: every distance of a score below
-its maximum, logits of every magnitude, finite masks."""
+its maximum, logits of every magnitude, finite masks, peaked rows."""
 import numpy as np
 import pytest
 import torch
@@ -137,3 +137,35 @@ def test_logprobs_rows_of_any_magnitude(cuda_ok):
     for k in range(-6, 39, 2):                             # a spread of that size
         x.append(r.uniform(-1, 1, V) * 3 * 10.0 ** k)
     check_rows(np.stack(x), [0, 9999, V - 1], top=20)
+
+
+def test_logprobs_two_entries_of_one_thread(cuda_ok):
+    """A row of two entries, the second 0.5 to 17 above the first and 8192 columns behind it: the smaller came first,
+    and what is left of the sum beside 1 is all that log(sum) and the entropy consist of."""
+    V = 16384
+    d = np.concatenate([np.linspace(0.5, 17, 200), [15.9, 15.95, 15.99]])
+    x = np.full((len(d), V), -np.inf)
+    x[:, 40], x[:, 40 + 8192] = 0.3, 0.3 + d
+    check_rows(x, [40, 40 + 8192], top=3)
+
+
+@pytest.mark.parametrize("V", [5000, 40001, 262144])
+def test_logprobs_peaked_rows(cuda_ok, V):
+    """One entry takes most of the row, anywhere in it; some of the others, or all, are far below."""
+    r = np.random.default_rng(3)
+    x = r.standard_normal((120, V))
+    x[:40, r.random(V) < 0.9] = -np.inf
+    x[40:80, r.random(V) < 0.9995] = -np.inf
+    at = r.integers(0, V, 120)
+    x[np.arange(120), at] = r.uniform(12, 16.9, 120)
+    x[::2] += r.uniform(-300, 300, (60, 1))
+    check_rows(x, [int(at[3]), int(at[50]), int(at[100]), 17], top=9)
+
+
+def test_logprobs_rising_and_falling_rows(cuda_ok):
+    """The maximum moves all along the row, by steps below and above 16."""
+    V = 70001
+    up = [np.linspace(-s, s, V) for s in (0.01, 1, 5, 12, 40, 300)]
+    steps = [np.floor(np.arange(V) / 4096) * s for s in (0.3, 3.0, 15.9, 16.1, 40.0)]
+    x = np.stack([y[::k] for y in up + steps for k in (1, -1)])
+    check_rows(x, [0, V // 2, V - 1], top=4)
