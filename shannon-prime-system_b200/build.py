@@ -31,7 +31,7 @@ NVFLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-rela
 CU_SRCS = ["spb_kernels.cu", "spb_gemm_tc.cu", "spb_runtime.cu", "spb_noalloc.cu", "spb_tp.cu",
            "spb_tree.cu", "spb_logprobs.cu"]
 HDRS = ["spb_exact.cuh", "spb_kernels.cuh", "spb_async.cuh", "spb_device.cuh", "spb_tp.cuh", "spb_spinor.cuh",
-        "spb_tree.cuh"]
+        "spb_tree.cuh", "spb_logprob_plan.h"]
 
 
 def _newer(out, deps):

@@ -26,8 +26,10 @@
 // equal in great number, can overflow that list: they find one entry after the other.
 #include <cooperative_groups.h>
 #include <cstdlib>
+#include <mutex>
 
 #include "spb_exact.cuh"
+#include "spb_logprob_plan.h"
 #include "spb_tree.cuh"
 
 namespace cg = cooperative_groups;
@@ -37,8 +39,6 @@ namespace spb {
 namespace {
 
 constexpr int LT = 512, LW = LT / 32;
-constexpr int LPART = 16384;       // entries of a part, up to 16 parts
-constexpr int LPARTS = 16;
 constexpr int LCAND = 2048;        // entries at or above the bound that are ranked by counting
 constexpr int LBATCH = 4;          // groups of four in flight per thread
 constexpr float LOG2E_F = 1.44269504f;
@@ -403,40 +403,58 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
   }
 }
 
+// which clusters run, asked once per device (a capture never sees a failed launch)
+struct Room {
+  std::once_flag once;
+  cudaError_t e = cudaSuccess;
+  bool fits[2][3][LPARTS + 1] = {};   // [entropy][pad][CTAs]
+};
+
+template <bool ENT>
+cudaError_t ask(bool (&fits)[3][LPARTS + 1]) {
+  cudaError_t e = cudaFuncSetAttribute(k_logprobs<ENT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<ENT>, cudaFuncAttributeMaxDynamicSharedMemorySize, LPADS[2]);
+  if (e != cudaSuccess) return e;
+  for (int p = 0; p < 3; p++)
+    for (int c = 2; c <= LPARTS; c++) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)c);
+      cfg.blockDim = dim3(LT);
+      cfg.dynamicSmemBytes = LPADS[p];
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = c;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      fits[p][c] = cudaOccupancyMaxActiveClusters(&n, k_logprobs<ENT>, &cfg) == cudaSuccess && n > 0;
+    }
+  (void)cudaGetLastError();
+  return cudaSuccess;
+}
+
 }  // namespace
 
 cudaError_t launch_logprobs(const LogprobArgs &a, cudaStream_t st) {
   if (a.rows <= 0) return cudaSuccess;
-  int P = (a.vocab + LPART - 1) / LPART;
-  if (P > LPARTS) P = LPARTS;
-  const int per = ((a.vocab + P - 1) / P + 3) & ~3;
-  P = (a.vocab + per - 1) / per;
-  // few rows: a row over as many CTAs as it has parts; more: over fewer, so that the call is one wave of two
-  // CTAs per SM (64 rows x 262144, 20 alternatives, at that step: 45 us with at most one per SM, 29 with two,
-  // 43 and 61 with two and four waves); many rows: a CTA each, three per SM
-  int C = P;
-  if ((long long)a.rows * C > 2 * 148) C = a.rows < 2 * 148 ? 2 * 148 / a.rows : 1;
-  const int each = (P + C - 1) / C;   // parts of a CTA, spread evenly
-  C = (P + each - 1) / each;
-  static bool set[64];
+  static Room rooms[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (!set[dev & 63]) {
-    e = cudaFuncSetAttribute(k_logprobs<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 92 * 1024);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_logprobs<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, 92 * 1024);
-    if (e != cudaSuccess) return e;
-    set[dev & 63] = true;
-  }
+  Room &room = rooms[dev & 63];
+  std::call_once(room.once, [&] {
+    room.e = ask<false>(room.fits[0]);
+    if (room.e == cudaSuccess) room.e = ask<true>(room.fits[1]);
+  });
+  if (room.e != cudaSuccess) return room.e;
+  const auto &fits = room.fits[a.entropy ? 1 : 0];
+  const LogprobPlan plan = plan_logprobs(a.rows, a.vocab, [&](int c, int pad) { return fits[pad == 0 ? 0 : pad == LPADS[1] ? 1 : 2][c]; });
+  const int C = plan.ctas, P = plan.parts, per = plan.per;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(C * a.rows));
   cfg.blockDim = dim3(LT);
-  // calls of one wave spread over all SMs: unused shared memory keeps a second (third) CTA off an SM, where
-  // the scheduler would fill it first (64 rows: 30 -> 26 us)
-  const long long ctas = (long long)a.rows * C;
-  cfg.dynamicSmemBytes = ctas <= 148 ? 92 * 1024 : ctas <= 2 * 148 ? 52 * 1024 : 0;
+  cfg.dynamicSmemBytes = plan.pad;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   int na = 0;
