@@ -831,7 +831,8 @@ static void release_pages(spb_session *s) {
 
 // Make positions [pos, pos + n) writable: every page they touch becomes this session's alone (a
 // fresh page, or a copy of a page another session still holds), then the device page table
-// follows. A copy is waited for before the other holder may write its page in place again.
+// follows. A pool without that many free pages is left as it was, and so are the session's pages.
+// A copy is waited for before the other holder may write its page in place again.
 static int prepare_write(spb_session *s, int pos, int n) {
   spb_kvpool *pool = s->pool;
   s->n_tree = 0;   // a drafted tree behind the context is written over
@@ -840,11 +841,14 @@ static int prepare_write(spb_session *s, int pos, int n) {
   bool changed = false, copied = false;
   {
     std::lock_guard<std::mutex> lk(pool->mu);
-    for (int j = pos / pool->pg; j <= (pos + n - 1) / pool->pg; j++) {
-      const int cur = s->pages[j];
-      if (cur >= 0 && pool->refs[cur] == 1) continue;
-      if (pool->free_list.empty()) return set_err(SPB_EOOM, "spb: the KV page pool has no free page");
-      const int np = pool->free_list.back();
+    const int j0 = pos / pool->pg, j1 = (pos + n - 1) / pool->pg;
+    const auto own = [&](int j) { return s->pages[j] >= 0 && pool->refs[s->pages[j]] == 1; };
+    size_t need = 0;
+    for (int j = j0; j <= j1; j++) need += !own(j);
+    if (need > pool->free_list.size()) return set_err(SPB_EOOM, "spb: the KV page pool has no free page");
+    for (int j = j0; j <= j1; j++) {
+      if (own(j)) continue;
+      const int cur = s->pages[j], np = pool->free_list.back();
       pool->free_list.pop_back();
       pool->refs[np] = 1;
       if (cur >= 0) {   // shared: copy before writing
