@@ -1,11 +1,11 @@
 """Values at which the kernels that verify drafted trees can go wrong: every distance of a score below
-its maximum, logits of every magnitude, finite masks, peaked rows."""
+its maximum, contexts that go in runs, logits of every magnitude, finite masks, peaked rows."""
 import numpy as np
 import pytest
 import torch
 
 import spb200
-from test_gpu_tree import dev, errs, exp_fixed, run_lp, u32
+from test_gpu_tree import Case, chain, dev, errs, exp_fixed, run_lp, tree, u32
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +169,80 @@ def test_logprobs_rising_and_falling_rows(cuda_ok):
     steps = [np.floor(np.arange(V) / 4096) * s for s in (0.3, 3.0, 15.9, 16.1, 40.0)]
     x = np.stack([y[::k] for y in up + steps for k in (1, -1)])
     check_rows(x, [0, V // 2, V - 1], top=4)
+
+
+def attend_far(K, V, q, ctx, parent, win, G):
+    """The contract (`attend`) for long contexts: V in digits of 10 bits, so that the sums fit int64."""
+    n, NKV, HD = len(parent), K.shape[1], K.shape[2]
+    asc = np.float32(1.0) / np.sqrt(np.float32(HD))
+    out = np.zeros((n, NKV, G, HD), np.float32)
+    for i in range(n):
+        c = chain(parent, i)
+        first = max(0, ctx + len(c) - win) if win > 0 else 0
+        see = np.array(list(range(min(first, ctx), ctx)) + [ctx + a for t, a in enumerate(c) if ctx + t >= first])
+        for g in range(NKV):
+            k, v = K[see, g].astype(np.int64), V[see, g].astype(np.int64)
+            v0, v1, v2 = v & 1023, (v >> 10) & 1023, v >> 20
+            for h in range(G):
+                s = (k * q[i].reshape(NKV, G, HD)[g, h].astype(np.int64)).sum(1)
+                z = ((s.astype(np.float64) * 2.0 ** -32).astype(np.float32) * asc).astype(np.float64) * 16384.0
+                zi = np.where(z < 0, np.ceil(z - 0.5), np.floor(z + 0.5)).astype(np.int64)
+                e = exp_fixed(zi.max() - zi)
+                S, N = int(e.sum()), [(e @ d).tolist() for d in (v0, v1, v2)]
+                out[i, g, h] = [np.float32(float(((a + (b << 10) + (c2 << 20)) << 16) // S) * 2.0 ** -32) for a, b, c2 in zip(*N)]
+    return out.reshape(n, NKV * G * HD)
+
+
+def want_far(c, win=-1):
+    res = []
+    for b, ctx in enumerate(c.ctx):
+        slots = np.arange(ctx + len(c.trees[b]))
+        pg, at = c.tab[b, slots // c.page], slots % c.page
+        res.append(attend_far(c.k[pg, c.layer, :, at], c.v[pg, c.layer, :, at], c.q[c.row0[b]:c.row0[b + 1]], ctx, c.trees[b], win, c.G))
+    return np.concatenate(res)
+
+
+def outliers(c):
+    """Some entries at the grid's limits: their fourth digits are not zero."""
+    lim = c.r.random(c.k.shape[:-1]) < 0.002
+    c.k[lim, 3], c.v[lim, 5] = (1 << 24) - 1, -(1 << 30) + 1
+    c.q[:, 3] = 1000
+    return c
+
+
+@pytest.mark.parametrize("HD,G,page,ctx,nodes", [
+    (64, 2, 128, 34000, 3), (128, 1, 4096, 34000, 3), (256, 1, 128, 34000, 2), (64, 1, 1000, 70000, 3), (128, 2, 128, 70000, 2),
+    (256, 1, 4096, 70000, 3),
+])
+def test_attention_in_runs(cuda_ok, HD, G, page, ctx, nodes):
+    """More slots than a cluster of CTAs keeps scores for (16 x 2112): maxima first, then run after run."""
+    c = outliers(Case(13, 1, G, HD, page, [ctx], [tree(np.random.default_rng(1), nodes, 0.7)])).upload()
+    errs()
+    got = c.run().cpu().numpy()
+    assert errs() == 0
+    assert np.array_equal(u32(got), u32(want_far(c)))
+
+
+@pytest.mark.parametrize("HD", [64, 128, 256])
+def test_attention_in_runs_of_ragged_sequences(cuda_ok, HD):
+    """Long, short and empty contexts, and a sequence without nodes, in one call; 32 heads' worth of nodes."""
+    r = np.random.default_rng(2)
+    ctx, nodes = [500, 35001, 0, 1056, 77], [20, 2, 5, 0, 1]
+    c = outliers(Case(14, 2, 2, HD, 96, ctx, [tree(r, n, 0.5) for n in nodes])).upload()
+    assert np.array_equal(u32(c.run().cpu().numpy()), u32(want_far(c)))
+
+
+@pytest.mark.parametrize("HD,win", [(64, 35000), (256, 34000)])
+def test_attention_in_runs_of_a_window(cuda_ok, HD, win):
+    c = outliers(Case(15, 1, 2, HD, 128, [40000], [[-1, 0, 1, -1]])).upload()
+    assert np.array_equal(u32(c.run(win=win).cpu().numpy()), u32(want_far(c, win)))
+
+
+@pytest.mark.parametrize("HD", [64, 128, 256])
+@pytest.mark.parametrize("nodes,ctx", [(64, 300), (7, 5000)])
+def test_attention_in_runs_or_not(cuda_ok, HD, nodes, ctx):
+    """A call that allows for long contexts gives short ones the same bytes."""
+    c = outliers(Case(16, 2, 2, HD, 64, [ctx, 40], [tree(np.random.default_rng(3), n, 0.6) for n in (nodes, 3)])).upload()
+    one = c.run().cpu().numpy()
+    for far in (33729, 200000, 1048512):
+        assert np.array_equal(u32(c.run(max_ctx=far).cpu().numpy()), u32(one))
