@@ -832,14 +832,16 @@ static void release_pages(spb_session *s) {
 // Make positions [pos, pos + n) writable: every page they touch becomes this session's alone (a
 // fresh page, or a copy of a page another session still holds), then the device page table
 // follows. A pool without that many free pages is left as it was, and so are the session's pages.
-// A copy is waited for before the other holder may write its page in place again.
+// A copied page counts this session as a holder until the copy is done: before that another thread's
+// session must not write the page in place, nor a close hand it on.
 static int prepare_write(spb_session *s, int pos, int n) {
   spb_kvpool *pool = s->pool;
   s->n_tree = 0;   // a drafted tree behind the context is written over
   if (!pool || n <= 0) return SPB_OK;
   if (pos < 0 || pos + n > s->pmax) return set_err(SPB_ECONTEXT_FULL, "spb: context full");
-  bool changed = false, copied = false;
+  bool changed = false;
   {
+    std::vector<int32_t> copied;
     std::lock_guard<std::mutex> lk(pool->mu);
     const int j0 = pos / pool->pg, j1 = (pos + n - 1) / pool->pg;
     const auto own = [&](int j) { return s->pages[j] >= 0 && pool->refs[s->pages[j]] == 1; };
@@ -857,16 +859,16 @@ static int prepare_write(spb_session *s, int pos, int n) {
                            cudaMemcpyDeviceToDevice, s->st));
         CU(cudaMemcpyAsync(pool->v + (size_t)np * pool->page_elems, pool->v + (size_t)cur * pool->page_elems, bytes,
                            cudaMemcpyDeviceToDevice, s->st));
-        pool->refs[cur]--;
-        copied = true;
+        copied.push_back(cur);
       }
       s->pages[j] = np;
       changed = true;
     }
+    if (!copied.empty()) CU(cudaStreamSynchronize(s->st));
+    for (int32_t pg : copied) pool->refs[pg]--;
   }
   if (changed)
     CU(cudaMemcpyAsync(s->ptab_dev, s->pages.data(), s->pages.size() * 4, cudaMemcpyHostToDevice, s->st));
-  if (copied) CU(cudaStreamSynchronize(s->st));
   return SPB_OK;
 }
 

@@ -1,4 +1,6 @@
-"""Sessions with drafted trees where the calls around them matter: page pools that run out."""
+"""Sessions with drafted trees where the calls around them matter: page pools that run out, threads."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 
@@ -38,5 +40,41 @@ def test_a_step_without_room_changes_nothing(xr, cuda_ok):
     for h in (s, c, t, xs, xc, xt):
         h.close()
     assert pool.free_pages() == 3
+    pool.free()
+    m.free()
+
+
+def test_sessions_that_share_pages_on_two_threads(cuda_ok):
+    """Two sessions forked from one prompt write their first positions, trees and steps, on threads of their own:
+    the copy of the page they share is done before the other one writes it."""
+    cfg = spmodel.CONFIGS["micro_gemma"]
+    m = spb200.Model.upload(cfg, spmodel.gen_model(cfg, seed=5))
+    pool = spb200.KvPool(m, 128, 8)
+    prompt = spmodel.gen_tokens(62, 100, cfg.n_vocab)
+
+    def go(h, first):
+        res = h.tree_step([first, first + 1, first + 2], [-1, 0, 0])
+        rows = [res.logits.copy()]
+        h.tree_commit([0, 2])
+        rows += [h.step(first + 3 + i).copy()[None] for i in range(3)]
+        return np.concatenate(rows)
+
+    def fork():
+        a = pool.session(300)
+        a.prefill(prompt, logits=False)
+        return a, a.clone()
+
+    a, b = fork()
+    want = [go(a, 5), go(b, 50)]
+    a.close()
+    b.close()
+    with ThreadPoolExecutor(2) as ex:
+        for _ in range(40):
+            hs = fork()
+            got = list(ex.map(go, hs, (5, 50)))
+            for g, w, h in zip(got, want, hs):
+                assert np.array_equal(u32(g), u32(w))
+                h.close()
+    assert pool.free_pages() == 8
     pool.free()
     m.free()
