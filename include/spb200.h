@@ -283,8 +283,9 @@ int spb_kv_compact(const spb_kv_view *kv, int n_seq, const int32_t *ctx, const i
  * and entropy 0; a row with NaN or +inf has no distribution: NaN, ids -1. A row's bytes depend neither on
  * the other rows of the call nor on its alignment. vocab at most 4194304, rows and n_tok at
  * most 2^26 (SPB_EUNSUPPORTED). Device buffers of the current device that overlap nowhere; no workspace, calls
- * on different streams are independent (a first call before any capture, as above). Every row looks through
- * the list of tokens: with tok_row, longer lists than a row has entries are better cut by rows. */
+ * on different streams are independent (a first call before any capture, as above). With tok_row every row
+ * looks through the list of tokens: lists longer than a row has entries are better cut by rows, and rows x n_tok
+ * is at most 2^40 (SPB_EUNSUPPORTED). */
 int spb_logprobs(const float *logits, int rows, int vocab, int64_t ld, const int32_t *tok_row,
                  const int32_t *tok, int n_tok, float *logprob, float *lse, float *entropy, int top,
                  int32_t *top_id, float *top_logprob, void *stream);

@@ -1892,6 +1892,9 @@ extern "C" int spb_logprobs(const float *logits, int rows, int vocab, int64_t ld
   if (top < 0 || top > LOGPROB_TOP) return set_err(SPB_EBADARG, "spb_logprobs: top in [0, %d]", LOGPROB_TOP);
   if (vocab > LOGPROB_VOCAB || rows > (1 << 26) || n_tok > (1 << 26))
     return set_err(SPB_EUNSUPPORTED, "spb_logprobs: %d entries per row, 2^26 rows and 2^26 tokens at most", LOGPROB_VOCAB);
+  // with tok_row every row looks through the list, 10^12 (row, token) pairs a second: a second at most
+  if (tok_row && (int64_t)rows * n_tok > (int64_t)1 << 40)
+    return set_err(SPB_EUNSUPPORTED, "spb_logprobs: 2^40 rows x tokens at most with tok_row (cut the call by rows)");
   if (rows == 0 && n_tok == 0) return SPB_OK;
   if (rows == 0 || !logits || (n_tok > 0 && (!tok || !logprob)) || (top > 0 && (!top_id || !top_logprob)))
     return set_err(SPB_EBADARG, "spb_logprobs: null arg, or tokens without rows");

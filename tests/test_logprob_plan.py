@@ -33,3 +33,16 @@ def test_logprob_clusters_that_do_not_fit(tmp_path):
             assert (ctas - 1) * -(-parts // ctas) < parts         # every CTA has a part
         if plans[16, 16][2] > 5:
             assert plans[8, 0][2] > 2 and plans[8, 0][3] == 0 and plans[1, 1][2] == 1
+
+
+def test_tokens_times_rows_are_limited():
+    """With tok_row every row looks through the list: a call that would take minutes is refused; without, none is."""
+    def call(rows, n_tok, tok_row=256):
+        try:
+            spb200.logprobs(256, rows, 8, 8, tok_row, 256, n_tok, 256, None, None, 0, None, None)
+        except spb200.SpbError as e:
+            return e.code
+    for rows, n_tok in ((1 << 26, 1 << 26), ((1 << 20) + 1, 1 << 20), (1 << 26, (1 << 14) + 1)):
+        assert call(rows, n_tok) == spb200.SPB_EUNSUPPORTED
+    for rows, n_tok, tok_row in ((1 << 20, 1 << 20, 256), (1 << 26, 1 << 14, 256), (1 << 26, 1 << 26, None)):
+        assert call(rows, n_tok, tok_row) == spb200.SPB_EBADARG      # (only its pointers are bad)
