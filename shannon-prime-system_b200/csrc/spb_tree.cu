@@ -172,8 +172,10 @@ __device__ __forceinline__ float finish(const acc128 &N, uint64_t S, double r) {
 // in), a row's pieces fetched by neighbouring lanes and shuffled (214, small trees 2 to 4 % slower), whole lines
 // of V by two neighbouring warps that hand each other their planes (290: a barrier per step), 16 slots per warp
 // and step of K (262), K in runs of four steps, in two buffers (spills) or in one (217 both).
+// 128 registers a thread at 16 warps hold all but 244 (width 256), 280 (128) and 312 bytes (64), which spill.
 // MULTI (more slots per rank than scores are kept for): the maxima first, then scores again in runs of
-// CS slots, each run's V-sums added up in shared memory.
+// CS slots, each run's V-sums added up in shared memory: K is read twice (12B shape, 4 nodes: 222 us behind
+// 33000 positions in one run, 476 behind 40000; 264 to 268 bytes spill, 216 at width 64).
 template <int HD, bool MULTI>
 struct TreeTile {
   static constexpr int QV = 16, KS = HD / 32;
