@@ -8,10 +8,12 @@
 //
 // One pass over the logits, so memory bounds it: 1000 rows x 151936 take 110 to 114 us, 81 to 85 % of the
 // measured copy rate; 64 rows x 262144 16.4 us (62 %; 256 CTAs on 148 SMs make up 1.6 of the 6.2 us above the
-// copy), 19.8 with one alternative and 23.1 with 20: every CTA ranks its own best, then they are joined. A row is cut into up to 16 parts of at least 16384 entries; a CTA's thread takes every 512th group of four
-// neighbours of a part, a warp joins its threads' sums, and a part its sixteen warps'. A cluster of C CTAs shares the parts of a row; C follows from the rows of the
-// call (few rows: a row over many CTAs), but what is summed in which order follows from the vocabulary's
-// size alone, so a row's bytes depend neither on the other rows nor on its alignment.
+// copy), 19.8 with one alternative and 23.1 with 20: every CTA ranks its own best, then they are joined. A row
+// is cut into up to 16 parts of at least 16384 entries; a CTA's thread takes every 512th group of four
+// neighbours of a part, a warp joins its threads' sums, and a part its sixteen warps'. A cluster of C CTAs
+// shares the parts of a row; C follows from the rows of the call (few rows: a row over many CTAs), but what is
+// summed in which order follows from the vocabulary's size alone, so a row's bytes depend neither on the other
+// rows nor on its alignment.
 //
 // A thread sums e^(x - m) = 2^((x - m) L), L = log2(e) in f32, and the same weighted by the exponents, with m
 // the largest entry it has met: so the row's largest entry counts 1 exactly, sum e >= 1, and neither log(sum e) nor
@@ -406,8 +408,8 @@ __global__ void __launch_bounds__(LT, 3) k_logprobs(LogprobArgs a, int C, int P,
 
 // which clusters run, asked once per device (a capture never sees a failed launch)
 struct Room {
-  std::once_flag once;
-  cudaError_t e = cudaSuccess;
+  std::mutex mu;
+  bool asked = false;                 // (a call that could not ask leaves it to the next)
   bool fits[2][3][LPARTS + 1] = {};   // [entropy][pad][CTAs]
 };
 
@@ -444,11 +446,15 @@ cudaError_t launch_logprobs(const LogprobArgs &a, cudaStream_t st) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   Room &room = rooms[dev & 63];
-  std::call_once(room.once, [&] {
-    room.e = ask<false>(room.fits[0]);
-    if (room.e == cudaSuccess) room.e = ask<true>(room.fits[1]);
-  });
-  if (room.e != cudaSuccess) return room.e;
+  {
+    std::lock_guard<std::mutex> lk(room.mu);
+    if (!room.asked) {
+      e = ask<false>(room.fits[0]);
+      if (e == cudaSuccess) e = ask<true>(room.fits[1]);
+      if (e != cudaSuccess) return e;
+      room.asked = true;
+    }
+  }
   const auto &fits = room.fits[a.entropy ? 1 : 0];
   const LogprobPlan plan = plan_logprobs(a.rows, a.vocab, [&](int c, int pad) { return fits[pad == 0 ? 0 : pad == LPADS[1] ? 1 : 2][c]; });
   const int C = plan.ctas, P = plan.parts, per = plan.per;
