@@ -20,8 +20,9 @@
 // x - m holds digits that the other has to cancel (a reference below the maximum costs a likely token's log
 // probability and a peaked row's entropy 1e-6).
 // The difference comes first: in x L - m L the rounding of m L grows with m (0.5 at 1e7, 2^99 at 1e37) and would
-// stand in the exponent. The exponential is ex2.approx, 2 units in the last place: entropies of 5 nats come out
-// 4e-7 low on the whole (exp2f 133 us and log2(e) in two parts 118 for the 1000 rows, both as low).
+// stand in the exponent. The exponential is ex2.approx, which is low on the whole by less than its 2 units in the
+// last place: entropies of 5 nats come out 4e-7 low (2e-8 with a double's exponential; exp2f, 133 us for the 1000
+// rows, and log2(e) in two parts, 118, are as low).
 //
 // The largest entries: the top'th largest of the threads' maxima bounds the top'th largest entry from below,
 // and only the threads that reach it can hold larger ones: their groups are read again (from L2) and what
